@@ -40,7 +40,7 @@ def listed():
         product("one token, square", 1, 4096, 4096, "f16"),                       # a decode step's attention projection: latency
         product("one token, wide", 1, 28672, 8192, "bf16"),                       # a decode step's gate or up projection: one read of W
         product("16 tokens, long k", 16, 8192, 28672, "bf16"),                    # a decode batch's down projection
-        product("odd sizes", 77, 1001, 1040, "f32", bias=True),                   # a small head: N no multiple of 4, a part of a block in K
+        product("odd sizes", 77, 1001, 1040, "bf16", bias=True),                  # a small head: N no multiple of 4, a part of a block in K
         product("ragged batch", 333, 11008, 4096, "f16", a="e5m2", bias=True),    # sequences packed without padding; wide-range activations
         product("prefill", 4096, 28672, 8192, "bf16"),                            # a prompt through the gate or up projection
         quantise("decode gate", 16, 28672, "bf16", gated=True),                   # silu(gate) * up in front of the down projection, decode
@@ -64,7 +64,7 @@ def draw(rng):
             if M * N * K <= 4096 * 28672 * 8192 and N * K <= 28672 * 8192:
                 break
         return {"op": op, "M": M, "N": N, "K": K, "a": rng.choice(["e4m3", "e4m3", "e5m2"]), "w": rng.choice(["e4m3", "e4m3", "e5m2"]),
-                "out": rng.choice(["f16", "bf16", "f32"]), "bias": rng.random() < 0.5}
+                "out": rng.choice(["f16", "bf16"]), "bias": rng.random() < 0.5}
     if op == "quantise":
         M, K = _log(rng, 1, 4096), _log(rng, 64, 28672)
         tile = rng.random() < 0.3
