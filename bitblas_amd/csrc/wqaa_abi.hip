@@ -12,6 +12,7 @@
 
 #include <mutex>
 
+#include "wqaa_block.h"
 #include "wqaa_common.h"
 #include "wqaa_kinds.h"
 
@@ -68,6 +69,7 @@ static void ensure_device(int dev) {
       di.ok = 1;
       gemv_init();
       gemm_init();
+      block_init();
     } else {
       (void)hipGetLastError();
     }
@@ -663,6 +665,101 @@ int wqaa_act_quant_int8(const void* X, int64_t rows, int K, void* Q, float* S, v
     return WQAA_ERR_NO_DEVICE;
   }
   return act_quant_launch(X, rows, K, Q, S, reinterpret_cast<hipStream_t>(stream));
+}
+
+static bool valid_block_desc(const wqaa_block_desc* d) {
+  if (!d || d->struct_size != (int32_t)sizeof(wqaa_block_desc)) {
+    set_error(WQAA_ERR_BAD_DESC, "block_matmul: null descriptor, or one of another size (ABI mismatch)");
+    return false;
+  }
+  if (d->N <= 0 || d->K <= 0) {
+    set_error(WQAA_ERR_BAD_DESC, "block_matmul: N=%d K=%d must be positive", d->N, d->K);
+    return false;
+  }
+  auto fp8 = [](int t) { return t == WQAA_E4M3 || t == WQAA_E5M2; };
+  const bool out = d->out_dtype == WQAA_F16 || d->out_dtype == WQAA_BF16;
+  // K: the operands are read in 16-byte pieces, and a piece never crosses a row; 2^22: offsets inside a 256-row tile stay in 31 bits
+  if (!fp8(d->a_dtype) || !fp8(d->w_dtype) || !out || d->K % 16 != 0 || d->K > (1 << 22)) {
+    set_error(WQAA_ERR_UNSUPPORTED, "block_matmul: operands are e4m3 / e5m2, outputs float16 / bfloat16, K a multiple of 16 up to 2^22 (K=%d)", d->K);
+    return false;
+  }
+  return true;
+}
+
+int wqaa_block_matmul(const wqaa_block_desc* desc, const void* A, const void* W, const float* scale_a, int64_t scale_a_ld,
+                      const float* scale_w, const void* bias, void* C, int m, void* workspace, uint64_t workspace_bytes, void* stream) {
+  if (!valid_block_desc(desc)) return wqaa_last_error();
+  if (m == 0) return WQAA_OK;
+  if (m < 0 || !A || !W || !scale_a || !scale_w || !C || (desc->with_bias && !bias)) {
+    set_error(WQAA_ERR_BAD_DESC, "block_matmul: bad call (m=%d, or a null operand)", m);
+    return WQAA_ERR_BAD_DESC;
+  }
+  if (scale_a_ld < m || ((reinterpret_cast<uintptr_t>(A) | reinterpret_cast<uintptr_t>(W)) & 15)) {
+    set_error(WQAA_ERR_BAD_DESC, "block_matmul: scale_a_ld >= m, and A and W aligned to 16 bytes, are required");
+    return WQAA_ERR_BAD_DESC;
+  }
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  StreamDeviceScope scope(s, A);
+  if (!device_info().ok) {
+    set_error(WQAA_ERR_NO_DEVICE, "no HIP device visible");
+    return WQAA_ERR_NO_DEVICE;
+  }
+  const int st = block_gemm_launch(*desc, A, W, scale_a, scale_a_ld, scale_w, bias, C, m, workspace, workspace_bytes, s);
+  if (st == WQAA_OK) g_last_error = WQAA_OK;
+  return st;
+}
+
+uint64_t wqaa_block_workspace_bytes(const wqaa_block_desc* desc, int m) {
+  if (!valid_block_desc(desc) || m <= 0) return 0;
+  return block_gemm_workspace_bytes(*desc, m);
+}
+
+int wqaa_block_select(const wqaa_block_desc* desc, int m, wqaa_plan* plan) {
+  if (!valid_block_desc(desc)) return wqaa_last_error();
+  return block_gemm_plan(*desc, m <= 0 ? 1 : m, plan);
+}
+
+int wqaa_block_quantize(const wqaa_block_quant* q, void* stream) {
+  if (!q || q->struct_size != (int32_t)sizeof(wqaa_block_quant) || q->rows < 0 || q->K <= 0) {
+    set_error(WQAA_ERR_BAD_DESC, "block_quantize: malformed arguments");
+    return WQAA_ERR_BAD_DESC;
+  }
+  if (q->rows == 0) return WQAA_OK;
+  if (!q->X || !q->Q || !q->S || q->x_ld < q->K || (q->gate && q->gate_ld < q->K) || (!q->tile && q->s_ld < q->rows)) {
+    set_error(WQAA_ERR_BAD_DESC, "block_quantize: a null operand, or rows that overlap");
+    return WQAA_ERR_BAD_DESC;
+  }
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  StreamDeviceScope scope(s, q->X);
+  if (!device_info().ok) {
+    set_error(WQAA_ERR_NO_DEVICE, "no HIP device visible");
+    return WQAA_ERR_NO_DEVICE;
+  }
+  const int st = block_quantize_launch(*q, s);
+  if (st == WQAA_OK) g_last_error = WQAA_OK;
+  return st;
+}
+
+int wqaa_residual_norm(const wqaa_residual_norm_args* n, void* stream) {
+  if (!n || n->struct_size != (int32_t)sizeof(wqaa_residual_norm_args) || n->rows < 0 || n->D <= 0) {
+    set_error(WQAA_ERR_BAD_DESC, "residual_norm: malformed arguments");
+    return WQAA_ERR_BAD_DESC;
+  }
+  if (n->rows == 0) return WQAA_OK;
+  if (!n->x || (!n->stream && !n->Y) || (n->Y && !n->weight) || (n->Y && n->q_dtype >= 0 && (!n->S || n->s_ld < n->rows)) ||
+      n->x_ld < n->D || (n->residual && n->residual_ld < n->D) || (n->gate && (n->gate_rows <= 0 || n->gate_ld < 0))) {
+    set_error(WQAA_ERR_BAD_DESC, "residual_norm: a null operand, nothing to write, or rows that overlap");
+    return WQAA_ERR_BAD_DESC;
+  }
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  StreamDeviceScope scope(s, n->x);
+  if (!device_info().ok) {
+    set_error(WQAA_ERR_NO_DEVICE, "no HIP device visible");
+    return WQAA_ERR_NO_DEVICE;
+  }
+  const int st = residual_norm_launch(*n, s);
+  if (st == WQAA_OK) g_last_error = WQAA_OK;
+  return st;
 }
 
 int wqaa_select(const wqaa_matmul_desc* desc, int m, wqaa_plan* plan) {

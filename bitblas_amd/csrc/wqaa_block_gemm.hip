@@ -1,0 +1,123 @@
+// wqaa_block_gemm.hip - the block-scaled 8-bit product: which member a call takes, and its launch.
+#include "wqaa_block_gemm_kernel.h"
+
+namespace wqaa {
+
+namespace {
+
+struct Choice {
+  int stream_waves;      // > 0: the streaming member with this many waves
+  int bm;                // tile member: activation rows of a tile
+  int tiles_m, tiles_n, split, split_len;
+};
+
+Choice choose(const wqaa_block_desc& d, int m) {
+  Choice c = {};
+  const int kb = (d.K + kBlock - 1) / kBlock;
+  if (m <= 16) {
+    c.stream_waves = kb >= 16 ? 8 : 4;
+    c.tiles_m = 1, c.tiles_n = (d.N + 15) / 16, c.split = 1, c.split_len = kb;
+    return c;
+  }
+  c.bm = m <= 32 ? 32 : m <= 64 ? 64 : 128;
+  c.tiles_m = (m + c.bm - 1) / c.bm;
+  c.tiles_n = (d.N + kBlock - 1) / kBlock;
+  // fewer tiles than CUs: K in slices of at least 4 blocks, so that the slices fill the chip once
+  const long tiles = (long)c.tiles_m * c.tiles_n;
+  long split = tiles >= 256 ? 1 : 256 / tiles;
+  if (split > kb / 4) split = kb / 4;
+  if (split < 1) split = 1;
+  c.split_len = (int)((kb + split - 1) / split);
+  c.split = (kb + c.split_len - 1) / c.split_len;
+  return c;
+}
+
+template <class P>
+void tile_attr() {
+  (void)hipFuncSetAttribute(reinterpret_cast<const void*>(wq_block_tile_kernel<P>), hipFuncAttributeMaxDynamicSharedMemorySize, P::LDS);
+}
+template <class P>
+void tile_go(const BlockGemmArgs& a, hipStream_t s) {
+  wq_block_tile_kernel<P><<<dim3(a.tiles_m * a.tiles_n * a.split), dim3(P::THREADS), P::LDS, s>>>(a);
+}
+template <int WF, int AF>
+void init_pair() {
+  tile_attr<BlockTile<WF, AF, 32, 3>>();
+  tile_attr<BlockTile<WF, AF, 64, 3>>();
+  tile_attr<BlockTile<WF, AF, 128, 4>>();
+}
+template <int WF, int AF>
+void launch_pair(const Choice& c, const BlockGemmArgs& a, hipStream_t s) {
+  if (c.stream_waves == 8) wq_block_stream_kernel<WF, AF, 8><<<dim3(a.tiles_n), dim3(512), 0, s>>>(a);
+  else if (c.stream_waves == 4) wq_block_stream_kernel<WF, AF, 4><<<dim3(a.tiles_n), dim3(256), 0, s>>>(a);
+  else if (c.bm == 32) tile_go<BlockTile<WF, AF, 32, 3>>(a, s);
+  else if (c.bm == 64) tile_go<BlockTile<WF, AF, 64, 3>>(a, s);
+  else tile_go<BlockTile<WF, AF, 128, 4>>(a, s);
+}
+
+}  // namespace
+
+void block_init() {
+  init_pair<0, 0>();
+  init_pair<0, 1>();
+  init_pair<1, 0>();
+  init_pair<1, 1>();
+}
+
+size_t block_gemm_workspace_bytes(const wqaa_block_desc& d, int m) {
+  const Choice c = choose(d, m);
+  return c.split > 1 ? (size_t)c.split * m * d.N * 4 : 0;
+}
+
+int block_gemm_plan(const wqaa_block_desc& d, int m, wqaa_plan* plan) {
+  if (!plan) return WQAA_OK;
+  const Choice c = choose(d, m);
+  memset(plan, 0, sizeof(*plan));
+  plan->kernel_family = 2;
+  plan->block_m = c.stream_waves ? 16 : c.bm;
+  plan->block_n = c.stream_waves ? 16 : 128;
+  plan->block_k = kBlock;
+  plan->threads = c.stream_waves ? c.stream_waves * 64 : 256;
+  plan->grid = c.tiles_m * c.tiles_n * c.split;
+  plan->split_k = c.split;
+  snprintf(plan->name, sizeof(plan->name), "block_matmul_m%dn%dk%d_%sx%s_%s%dx%d%s", m, d.N, d.K, short_dtype(d.a_dtype), short_dtype(d.w_dtype),
+           c.stream_waves ? "stream" : "tile", plan->block_m, plan->block_n, c.split > 1 ? "_split" : "");
+  return WQAA_OK;
+}
+
+int block_gemm_launch(const wqaa_block_desc& d, const void* A, const void* W, const float* sa, int64_t sa_ld, const float* sw, const void* bias,
+                      void* C, int m, void* workspace, uint64_t workspace_bytes, hipStream_t stream) {
+  const Choice c = choose(d, m);
+  const uint64_t need = block_gemm_workspace_bytes(d, m);
+  if (need && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15))) {
+    set_error(WQAA_ERR_BAD_DESC, "block_matmul: m=%d needs %llu bytes of 16-byte aligned workspace", m, (unsigned long long)need);
+    return WQAA_ERR_BAD_DESC;
+  }
+  if ((long)c.tiles_m * c.tiles_n * c.split > 0x7fffffffl || (int64_t)m * 4 > 0x7fffffff) {
+    set_error(WQAA_ERR_UNSUPPORTED, "block_matmul: m=%d N=%d is too large", m, d.N);
+    return WQAA_ERR_UNSUPPORTED;
+  }
+  BlockGemmArgs a = {};
+  a.A = reinterpret_cast<const unsigned char*>(A), a.W = reinterpret_cast<const unsigned char*>(W);
+  a.sa = sa, a.sw = sw, a.sa_ld = sa_ld;
+  a.bias = d.with_bias ? bias : nullptr;
+  a.C = C, a.ws = reinterpret_cast<float*>(workspace);
+  a.M = m, a.N = d.N, a.K = d.K, a.KB = (d.K + kBlock - 1) / kBlock;
+  a.out_dtype = d.out_dtype;
+  a.tiles_m = c.tiles_m, a.tiles_n = c.tiles_n, a.split = c.split, a.split_len = c.split_len;
+  a.group_m = c.tiles_m < 8 ? c.tiles_m : 8;
+  const int wf = d.w_dtype == WQAA_E5M2, af = d.a_dtype == WQAA_E5M2;
+  if (wf == 0 && af == 0) launch_pair<0, 0>(c, a, stream);
+  else if (wf == 0) launch_pair<0, 1>(c, a, stream);
+  else if (af == 0) launch_pair<1, 0>(c, a, stream);
+  else launch_pair<1, 1>(c, a, stream);
+  if (c.split > 1) wq_block_reduce_kernel<<<dim3((unsigned)(((long)m * d.N + 255) / 256)), dim3(256), 0, stream>>>(a);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) {
+    set_error(WQAA_ERR_LAUNCH, "block_matmul: %s", hipGetErrorString(e));
+    return WQAA_ERR_LAUNCH;
+  }
+  return WQAA_OK;
+}
+
+}  // namespace wqaa

@@ -1,0 +1,279 @@
+// wqaa_block_gemm_kernel.h - the block-scaled 8-bit product:
+//     C[m, n] = sum_b sa[m, b] sw[n / 128, b] sum_{k in block b} a[m, k] w[n, k]
+// A block of 128 k is exactly one v_mfma_f32_16x16x128_f8f6f4, so the inner sum is one matrix instruction onto zero and the outer one
+// is four float32 fmas a lane with the block's scale.  The weights are the instruction's first operand: a lane then holds four
+// consecutive n of ONE row m (n = 4 (lane / 16) + i, m = lane % 16), its scale is one register for the whole fragment column, and
+// sw is the same for every n of a wave's weight rows (they lie inside one 128-row tile): sa sw is one product per fragment column.
+// Precision: the instruction adds the 8 products of consecutive k with each cut off (towards zero) at 2^-13 of the power of two of the
+// largest one, and everything above that level in float32 (measured: a product 2^-13 below the largest of its group of 8 counts, one
+// 2^-14 below does not; across groups it counts down to 2^-23).  A result of ordinary data is good to 2^-14.8 in the 2-norm, a
+// rounding to float16 costs 2^-12: hence float16 and bfloat16 outputs, and none in float32.
+// Operand map of the instruction: lane (r = lane % 16, q = lane / 16) feeds row r and 32 of the 128 k; which 32 is free as long as
+// both operands agree - here the 16-byte pieces q and 4 + q of the row's 128 bytes.
+#pragma once
+#include "wqaa_block.h"
+
+namespace wqaa {
+
+typedef float bf32x4 __attribute__((ext_vector_type(4)));
+typedef int bi32x4 __attribute__((ext_vector_type(4)));
+typedef int bi32x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t bu32x2 __attribute__((ext_vector_type(2)));
+
+// FMT: 0 e4m3, 1 e5m2 (the instruction's format fields); first operand W, second A
+template <int WF, int AF>
+__device__ __forceinline__ bf32x4 block_mfma(const bi32x4 (&w)[2], const bi32x4 (&a)[2]) {
+  const bi32x8 wv = {w[0][0], w[0][1], w[0][2], w[0][3], w[1][0], w[1][1], w[1][2], w[1][3]};
+  const bi32x8 av = {a[0][0], a[0][1], a[0][2], a[0][3], a[1][0], a[1][1], a[1][2], a[1][3]};
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wv, av, bf32x4{0.f, 0.f, 0.f, 0.f}, WF, AF, 0, 0x7F7F7F7F, 0, 0x7F7F7F7F);
+}
+
+__device__ __forceinline__ uint16_t block_bf16(float f) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, f);
+  if ((u & 0x7FFFFFFFu) > 0x7F800000u) return (uint16_t)((u >> 16) | 0x40u);
+  return (uint16_t)((u + 0x7FFFu + ((u >> 16) & 1u)) >> 16);
+}
+__device__ __forceinline__ float block_bias(const void* bias, int dt, int n) {
+  if (dt == WQAA_F16) return (float)reinterpret_cast<const _Float16*>(bias)[n];
+  return __builtin_bit_cast(float, (uint32_t)reinterpret_cast<const uint16_t*>(bias)[n] << 16);
+}
+__device__ __forceinline__ void block_store1(void* C, int dt, long i, float v) {
+  if (dt == WQAA_F16) reinterpret_cast<_Float16*>(C)[i] = (_Float16)v;
+  else reinterpret_cast<uint16_t*>(C)[i] = block_bf16(v);
+}
+
+// ---- m <= 16: the weights stream through registers --------------------------------------------------------------------------------
+// One read of W is all there is to do, so nothing is shared and nothing is staged: a wave takes 16 weight rows and every WAVES-th
+// k-block of them straight into the matrix operand's registers (two 16-byte loads a lane), the activations - one fragment of 16 rows, from
+// L2 - the same way; the waves' partial tiles meet in LDS in a fixed order.  Rows beyond m and n repeat the last one and are not stored.
+template <int WF, int AF, int WAVES>
+__global__ void __launch_bounds__(WAVES * 64) wq_block_stream_kernel(const BlockGemmArgs a) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  __shared__ float part[WAVES][256];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r = lane & 15, q = lane >> 4;
+  const int n0 = blockIdx.x * 16;
+  const unsigned char* wp = a.W + (long)min(n0 + r, a.N - 1) * a.K + q * 16;
+  const int m = min(r, a.M - 1);
+  const unsigned char* ap = a.A + (long)m * a.K + q * 16;
+  const float* swp = a.sw + (long)(n0 / kBlock) * a.KB;
+  const float* sap = a.sa + m;
+  bf32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  const int full = a.K / kBlock;                 // blocks that are whole
+  constexpr int U = 4;
+  int b = wave;
+  for (; b + (U - 1) * WAVES < full; b += U * WAVES) {
+    bi32x4 w[U][2], x[U][2];
+    float s[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const long k = (long)(b + u * WAVES) * kBlock;
+      w[u][0] = *reinterpret_cast<const bi32x4*>(wp + k);
+      w[u][1] = *reinterpret_cast<const bi32x4*>(wp + k + 64);
+      x[u][0] = *reinterpret_cast<const bi32x4*>(ap + k);
+      x[u][1] = *reinterpret_cast<const bi32x4*>(ap + k + 64);
+      s[u] = sap[(long)(b + u * WAVES) * a.sa_ld] * swp[b + u * WAVES];
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const bf32x4 d = block_mfma<WF, AF>(w[u], x[u]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[i] = __builtin_fmaf(d[i], s[u], acc[i]);
+    }
+  }
+  for (; b < a.KB; b += WAVES) {
+    const long k = (long)b * kBlock;
+    const int left = a.K - b * kBlock - q * 16;  // pieces beyond K are zero in both operands
+    bi32x4 w[2] = {}, x[2] = {};
+    if (left > 0) w[0] = *reinterpret_cast<const bi32x4*>(wp + k), x[0] = *reinterpret_cast<const bi32x4*>(ap + k);
+    if (left > 64) w[1] = *reinterpret_cast<const bi32x4*>(wp + k + 64), x[1] = *reinterpret_cast<const bi32x4*>(ap + k + 64);
+    const float s = sap[(long)b * a.sa_ld] * swp[b];
+    const bf32x4 d = block_mfma<WF, AF>(w, x);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[i] = __builtin_fmaf(d[i], s, acc[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) part[wave][r * 16 + q * 4 + i] = acc[i];
+  __syncthreads();
+  for (int t = threadIdx.x; t < 256; t += WAVES * 64) {
+    const int mm = t >> 4, n = n0 + (t & 15);
+    if (mm >= a.M || n >= a.N) continue;
+    float v = 0.f;
+#pragma unroll
+    for (int wv = 0; wv < WAVES; ++wv) v += part[wv][t];
+    if (a.bias) v += block_bias(a.bias, a.out_dtype, n);
+    block_store1(a.C, a.out_dtype, (long)mm * a.N + n, v);
+  }
+#endif
+}
+
+// ---- m > 16: tiles of BM x 128 through LDS ------------------------------------------------------------------------------------------
+// Four waves, S stages of one k-block each, every byte by LDS-DMA.  A stage holds BM activation rows and 128 weight rows of 128 bytes,
+// 16-byte piece g of row r at slot g ^ ((r >> 1) & 7) (the lanes of an operand read then hit every bank twice, which is the rate),
+// and per wave the scales of its own activation rows (64 of them; rows beyond M read as zero).
+template <int WF_, int AF_, int BM_, int S_>
+struct BlockTile {
+  static constexpr int WF = WF_, AF = AF_, BM = BM_, BN = 128, S = S_, THREADS = 256;
+  static constexpr int WM = BM >= 64 ? 2 : 1, WN = 4 / WM;               // wave grid
+  static constexpr int MF = BM / WM / 16, NF = BN / WN / 16;             // fragments of a wave
+  static constexpr int A_BYTES = BM * 128, W_BYTES = BN * 128, SC_BYTES = 4 * 256;
+  static constexpr int STAGE = A_BYTES + W_BYTES + SC_BYTES;
+  static constexpr int AP = BM / 32, WP = BN / 32;                       // DMA pieces (8 rows) of a wave per stage
+  static constexpr int PIECES = AP + WP + 1;
+  static constexpr int LDS = S * STAGE;
+  static_assert(LDS <= 160 * 1024 && MF * 16 <= 64, "LDS budget; one DMA piece holds a wave's row scales");
+};
+
+template <int N>
+__device__ __forceinline__ void block_wait_vm() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
+template <class P>
+__global__ void __launch_bounds__(P::THREADS) wq_block_tile_kernel(const BlockGemmArgs a) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  typedef __attribute__((address_space(3))) void* lds_t;
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r = lane & 15, q = lane >> 4;
+  const int wm = wave / P::WN, wn = wave % P::WN;
+
+  // workgroup -> (slice, tile): the workgroups of an XCD (block index modulo 8) walk neighbouring tiles, group_m M-tiles per N-tile
+  int blk = blockIdx.x;
+  const int nblk = gridDim.x;
+  if ((nblk & 7) == 0) blk = (blk & 7) * (nblk >> 3) + (blk >> 3);
+  const int per_slice = a.tiles_m * a.tiles_n;
+  const int slice = blk / per_slice;
+  blk -= slice * per_slice;
+  const int per_group = a.group_m * a.tiles_n;
+  const int group = blk / per_group;
+  const int first_m = group * a.group_m;
+  const int gsz = min(a.group_m, a.tiles_m - first_m);
+  const int rem = blk - group * per_group;
+  const int m0 = (first_m + rem % gsz) * P::BM, n0 = rem / gsz * P::BN;
+
+  const int b_first = slice * a.split_len, b_end = min(a.KB, b_first + a.split_len);
+
+  // tile-relative buffers: the range ends with the matrix, so rows beyond it read as zero
+  const long a_bytes = (long)min(P::BM, a.M - m0) * a.K, w_bytes = (long)min(P::BN, a.N - n0) * a.K;
+  const auto a_rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(a.A + (long)m0 * a.K), 0, (int)a_bytes, 0x00020000);
+  const auto w_rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(a.W + (long)n0 * a.K), 0, (int)w_bytes, 0x00020000);
+  const int pr = lane >> 3;                                              // row of a piece
+  const int g0 = (lane & 7) ^ ((lane >> 4) & 7), g1 = g0 ^ 4;            // source granule of even / odd pieces
+  constexpr uint32_t OUT = 0xC0000000u;                                  // beyond every buffer: reads as zero
+  const int sm = m0 + wm * (P::MF * 16) + lane;                          // the row whose scale this lane fetches
+  const bool sm_ok = lane < P::MF * 16 && sm < a.M;
+  const int last = a.KB - 1;
+  const int tail = a.K - last * kBlock;                                  // k in the last block
+
+  auto stage = [&](int t, int slot) {
+    const int b = min(b_first + t, b_end - 1);                           // (beyond the slice: the last block again, never used)
+    unsigned char* base = smem + slot * P::STAGE;
+    const bool cut = b == last;
+    const uint32_t k0 = (cut && g0 * 16 >= tail) ? OUT : (uint32_t)(g0 * 16), k1 = (cut && g1 * 16 >= tail) ? OUT : (uint32_t)(g1 * 16);
+#pragma unroll
+    for (int j = 0; j < P::AP; ++j) {
+      const int row = wave * (P::BM / 4) + j * 8;
+      const uint32_t k = (row & 8) ? k1 : k0;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(a_rsrc, (lds_t)(base + row * 128), 16, k == OUT ? OUT : k + (uint32_t)(row + pr) * (uint32_t)a.K, b * kBlock, 0, 0);
+    }
+#pragma unroll
+    for (int j = 0; j < P::WP; ++j) {
+      const int row = wave * (P::BN / 4) + j * 8;
+      const uint32_t k = (row & 8) ? k1 : k0;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(w_rsrc, (lds_t)(base + P::A_BYTES + row * 128), 16, k == OUT ? OUT : k + (uint32_t)(row + pr) * (uint32_t)a.K, b * kBlock, 0, 0);
+    }
+    // this wave's row scales of the block, 4 bytes a lane
+    const auto s_rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(a.sa + (long)b * a.sa_ld), 0, 0x7FFFFFFF, 0x00020000);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(s_rsrc, (lds_t)(base + P::A_BYTES + P::W_BYTES + wave * 256), 4, sm_ok ? (uint32_t)sm * 4u : OUT, 0, 0, 0);
+  };
+
+  bf32x4 acc[P::MF][P::NF];
+#pragma unroll
+  for (int f = 0; f < P::MF; ++f)
+#pragma unroll
+    for (int g = 0; g < P::NF; ++g) acc[f][g] = bf32x4{0.f, 0.f, 0.f, 0.f};
+  const int swl = (r >> 1) & 7;
+  const int rd0 = r * 128 + ((q ^ swl) * 16), rd1 = r * 128 + (((4 + q) ^ swl) * 16);
+  const float* swp = a.sw + (long)(n0 / kBlock) * a.KB + b_first;
+
+  const int nt = b_end - b_first;
+#pragma unroll
+  for (int t = 0; t < P::S - 1; ++t) stage(t, t);
+  int slot = 0, fill = P::S - 1;
+  for (int t = 0; t < nt; ++t) {
+    block_wait_vm<(P::S - 2) * P::PIECES>();      // this wave's pieces of block t have landed (one kind of load in flight: in order)
+    __syncthreads();                              // everyone's have, and everyone is done with block t - 1, whose slot is filled next
+    stage(t + P::S - 1, fill);
+    const unsigned char* base = smem + slot * P::STAGE;
+    const float sw = swp[t];
+    bi32x4 w[P::NF][2];
+#pragma unroll
+    for (int g = 0; g < P::NF; ++g) {
+      const unsigned char* p = base + P::A_BYTES + (wn * P::NF + g) * 2048;
+      w[g][0] = *reinterpret_cast<const bi32x4*>(p + rd0);
+      w[g][1] = *reinterpret_cast<const bi32x4*>(p + rd1);
+    }
+#pragma unroll
+    for (int f = 0; f < P::MF; ++f) {
+      const unsigned char* p = base + (wm * P::MF + f) * 2048;
+      const bi32x4 x[2] = {*reinterpret_cast<const bi32x4*>(p + rd0), *reinterpret_cast<const bi32x4*>(p + rd1)};
+      const float s = reinterpret_cast<const float*>(base + P::A_BYTES + P::W_BYTES + wave * 256)[f * 16 + r] * sw;
+#pragma unroll
+      for (int g = 0; g < P::NF; ++g) {
+        const bf32x4 d = block_mfma<P::WF, P::AF>(w[g], x);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[f][g][i] = __builtin_fmaf(d[i], s, acc[f][g][i]);
+      }
+    }
+    slot = slot + 1 == P::S ? 0 : slot + 1;
+    fill = fill + 1 == P::S ? 0 : fill + 1;
+  }
+  block_wait_vm<0>();                             // no DMA into LDS outlives the workgroup
+
+#pragma unroll
+  for (int f = 0; f < P::MF; ++f) {
+    const int m = m0 + (wm * P::MF + f) * 16 + r;
+#pragma unroll
+    for (int g = 0; g < P::NF; ++g) {
+      const int n = n0 + (wn * P::NF + g) * 16 + q * 4;
+      if (m >= a.M || n >= a.N) continue;
+      const int cnt = min(4, a.N - n);
+      if (a.split > 1) {
+        float* o = a.ws + ((long)slice * a.M + m) * a.N + n;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (i < cnt) o[i] = acc[f][g][i];
+        continue;
+      }
+      float v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = acc[f][g][i] + (a.bias && i < cnt ? block_bias(a.bias, a.out_dtype, n + i) : 0.f);
+      const long at = (long)m * a.N + n;
+      if (cnt == 4 && (a.N & 3) == 0) {
+        uint16_t b[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) b[i] = a.out_dtype == WQAA_F16 ? __builtin_bit_cast(uint16_t, (_Float16)v[i]) : block_bf16(v[i]);
+        *reinterpret_cast<bu32x2*>(reinterpret_cast<uint16_t*>(a.C) + at) = bu32x2{b[0] | (uint32_t)b[1] << 16, b[2] | (uint32_t)b[3] << 16};
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (i < cnt) block_store1(a.C, a.out_dtype, at + i, v[i]);
+      }
+    }
+  }
+#endif
+}
+
+// partial sums of the K slices, in slice order
+__global__ void __launch_bounds__(256) wq_block_reduce_kernel(const BlockGemmArgs a) {
+  const long total = (long)a.M * a.N;
+  const long i = (long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= total) return;
+  float v = 0.f;
+  for (int z = 0; z < a.split; ++z) v += a.ws[z * total + i];
+  if (a.bias) v += block_bias(a.bias, a.out_dtype, (int)(i % a.N));
+  block_store1(a.C, a.out_dtype, i, v);
+}
+
+}  // namespace wqaa

@@ -43,6 +43,7 @@ EXPORTED_SYMBOLS = (
     "init", "wqaa_abi_version", "wqaa_device_count", "wqaa_matmul", "wqaa_matmul_timed",
     "wqaa_matmul_ex", "wqaa_matmul_opts", "wqaa_workspace_bytes", "wqaa_matmul_group", "wqaa_matmul_group_ex", "wqaa_group_plan", "wqaa_matmul_gate_up", "wqaa_gate_up_plan", "wqaa_matmul_chain", "wqaa_chain_plan", "wqaa_dequantize", "wqaa_tune", "wqaa_act_quant_int8", "wqaa_select", "wqaa_select_ex", "wqaa_pack_weight", "wqaa_unpack_weight", "wqaa_relayout_weight", "wqaa_debug_decode", "wqaa_debug_row_blocks", "wqaa_debug_tile_of_block",
     "wqaa_peer_alloc", "wqaa_peer_free", "wqaa_peer_export", "wqaa_peer_open", "wqaa_peer_close", "wqaa_peer_exchange",
+    "wqaa_block_matmul", "wqaa_block_workspace_bytes", "wqaa_block_select", "wqaa_block_quantize", "wqaa_residual_norm",
     "wqaa_last_error", "wqaa_last_error_string",
 )
 

@@ -415,6 +415,76 @@ int wqaa_peer_open(const void* handle64, void** ptr);
 int wqaa_peer_close(void* ptr);
 int wqaa_peer_exchange(const wqaa_peer_exchange_desc* desc, void* stream);
 
+/* ---- block-scaled 8-bit floating point: both operands in e4m3 / e5m2, one float32 scale per block of 128 consecutive k ----------
+ * C[m, n] = sum_b scale_a(m, b) scale_w(n / 128, b) sum_{k in block b} A[m, k] W[n, k]  (+ bias[n]), one rounding to out_dtype.
+ * A: (m, K) bytes, W: (N, K) bytes, both row-major; K a multiple of 16, the last block may hold fewer than 128 k; any N >= 1.
+ * scale_a: the scale of (row m, block b) at scale_a[b * scale_a_ld + m], scale_a_ld >= m (the rows of one block side by side: what
+ * wqaa_block_quantize writes); scale_w: (ceil(N / 128), ceil(K / 128)) row-major; bias: (N,) of out_dtype when with_bias.
+ * Sums are float32, but for the matrix unit's own: of 8 consecutive k it adds the products with what each has below 2^-13 of the largest
+ * one's power of two cut off - 2^-14 of the result or so, less than a rounding to out_dtype (float16, bfloat16).  Replaces nothing in the reference, whose fp8 matmuls carry no scales
+ * (ops/general_matmul/__init__.py:372-383).  Small m splits K over workgroups: partial sums go to `workspace` (16-byte aligned, at least
+ * wqaa_block_workspace_bytes(desc, m) bytes, not shared with another stream while the call runs). */
+typedef struct wqaa_block_desc {
+  int32_t struct_size;   /* = sizeof(wqaa_block_desc) */
+  int32_t N, K;
+  int32_t a_dtype, w_dtype;   /* WQAA_E4M3 / WQAA_E5M2 */
+  int32_t out_dtype;          /* WQAA_F16 / WQAA_BF16 */
+  int32_t with_bias;
+  int32_t reserved[1];        /* 0 */
+} wqaa_block_desc;
+
+int wqaa_block_matmul(const wqaa_block_desc* desc, const void* A, const void* W, const float* scale_a, int64_t scale_a_ld,
+                      const float* scale_w, const void* bias, void* C, int m, void* workspace, uint64_t workspace_bytes, void* stream);
+uint64_t wqaa_block_workspace_bytes(const wqaa_block_desc* desc, int m);
+int wqaa_block_select(const wqaa_block_desc* desc, int m, wqaa_plan* plan);
+
+/* Quantiser of the operands above.  Over a block (128 consecutive k of one row; tile = 1: of 128 rows) s = max(max|x|, 2^-40) / L with L the
+ * largest value of q_dtype (448, 57344); q = x / s, the float32 quotient, rounded to nearest even.  A block that holds an infinity or
+ * a NaN gets a scale that is not finite, and NaN in all its values.  gate != NULL: x = silu(gate) * X, in float32.
+ * X, gate: (rows, K) with rows x_ld / gate_ld elements apart; Q: (rows, K) bytes, contiguous; S: (row, block) at S[block * s_ld + row], s_ld >= rows,
+ * or, for tiles, (ceil(rows / 128), ceil(K / 128)) row-major (s_ld is not read).  Any K >= 1. */
+typedef struct wqaa_block_quant {
+  int32_t struct_size;   /* = sizeof(wqaa_block_quant) */
+  int32_t x_dtype;       /* WQAA_F16 / WQAA_BF16 / WQAA_F32, of X and gate */
+  int32_t q_dtype;       /* WQAA_E4M3 / WQAA_E5M2 */
+  int32_t tile;
+  int64_t rows, K, x_ld, gate_ld, s_ld;
+  const void* X;
+  const void* gate;
+  void* Q;
+  float* S;
+} wqaa_block_quant;
+
+int wqaa_block_quantize(const wqaa_block_quant* args, void* stream);
+
+/* The norms on both sides of a block and the residual add between them, one launch:
+ *     z = x                  or  x * rsqrt(mean(x^2) + eps) * post_weight
+ *     h = residual_scale * residual + scale * gate * z           (residual NULL: no first term; gate NULL: 1)
+ *     y = h * rsqrt(mean(h^2) + eps) * weight                    (of h before it is rounded; weight NULL: no y)
+ * in float32; stream (h) in stream_dtype, y in x_dtype, or quantised in blocks of 128 as wqaa_block_quantize does (q_dtype).
+ * x, gate: x_dtype; residual: stream_dtype; rows x_ld / residual_ld elements apart, the gate of row r at gate + (r / gate_rows) * gate_ld.
+ * weights: (D,) of weight_dtype.  stream, Y: contiguous rows of D.  stream may be the residual itself; stream NULL: h is not written.
+ * 1 <= D <= 32768.  (integration/BitNet/modeling_bitnet.py:89-104 is the norm, :839-860 the residual adds around it.) */
+typedef struct wqaa_residual_norm_args {
+  int32_t struct_size;   /* = sizeof(wqaa_residual_norm_args) */
+  int32_t x_dtype;       /* WQAA_F16 / WQAA_BF16 */
+  int32_t stream_dtype;  /* x_dtype or WQAA_F32: of residual and stream */
+  int32_t weight_dtype;  /* x_dtype or WQAA_F32: of weight and post_weight */
+  int32_t q_dtype;       /* -1: y in x_dtype; WQAA_E4M3 / WQAA_E5M2: Q and S */
+  float eps, scale, residual_scale;
+  int64_t rows, D, x_ld, residual_ld, gate_ld, gate_rows, s_ld;
+  const void* x;
+  const void* residual;
+  const void* gate;
+  const void* post_weight;
+  const void* weight;
+  void* stream;
+  void* Y;               /* y, or the 8-bit values */
+  float* S;              /* scale of (row, block) at S[block * s_ld + row] */
+} wqaa_residual_norm_args;
+
+int wqaa_residual_norm(const wqaa_residual_norm_args* args, void* stream);
+
 /* ---- error side channel ---------------------------------------------------------------------- */
 int wqaa_last_error(void);
 const char* wqaa_last_error_string(void);

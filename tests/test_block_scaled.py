@@ -1,0 +1,155 @@
+"""Block-scaled 8-bit path without a device: configurations, plans, refusals at the Python and the C boundary, row and gate layouts."""
+import ctypes
+
+import pytest
+import torch
+
+import bitblas_amd as bitblas
+from bitblas_amd import block_scaled as bs
+from bitblas_amd import lib as wlib
+
+
+def test_struct_sizes_match_header():
+    assert ctypes.sizeof(bs.BlockDesc) == 8 * 4
+    assert ctypes.sizeof(bs.BlockQuant) == 4 * 4 + 5 * 8 + 4 * 8
+    assert ctypes.sizeof(bs.ResidualNormArgs) == 8 * 4 + 7 * 8 + 8 * 8
+
+
+@pytest.mark.parametrize("kw", [dict(N=0, K=128), dict(N=128, K=120), dict(N=128), dict(N=128, K=128, A_dtype="float16"),
+                                dict(N=128, K=128, W_dtype="int8"), dict(N=128, K=128, out_dtype="float32"), dict(N=128.0, K=128)])
+def test_config_refusals(kw):
+    with pytest.raises(ValueError):
+        bitblas.BlockScaledMatmulConfig(**kw)
+
+
+def _desc(**kw):
+    d = bs.BlockDesc()
+    d.struct_size = ctypes.sizeof(bs.BlockDesc)
+    d.N, d.K, d.a_dtype, d.w_dtype, d.out_dtype = 256, 256, wlib.E4M3, wlib.E4M3, wlib.F16
+    for k, v in kw.items():
+        setattr(d, k, v)
+    return d
+
+
+@pytest.mark.parametrize("kw, code", [(dict(struct_size=4), wlib.ERR_BAD_DESC), (dict(N=0), wlib.ERR_BAD_DESC), (dict(K=-16), wlib.ERR_BAD_DESC),
+                                      (dict(K=24), wlib.ERR_UNSUPPORTED), (dict(a_dtype=wlib.F16), wlib.ERR_UNSUPPORTED),
+                                      (dict(w_dtype=wlib.I8), wlib.ERR_UNSUPPORTED), (dict(out_dtype=wlib.F32), wlib.ERR_UNSUPPORTED),
+                                      (dict(K=(1 << 22) + 16), wlib.ERR_UNSUPPORTED)])
+def test_product_descriptor_refusals(kw, code):
+    L = bs._library()
+    d = _desc(**kw)
+    p = 4096
+    assert L.wqaa_block_matmul(ctypes.byref(d), p, p, p, 8, p, None, p, 8, None, 0, None) == code
+    assert L.wqaa_block_select(ctypes.byref(d), 8, None) == code
+    assert L.wqaa_block_workspace_bytes(ctypes.byref(d), 8) == 0
+
+
+def test_product_call_refusals():
+    L = bs._library()
+    p = 4096
+    d = _desc()
+    ok = [ctypes.byref(d), p, p, p, 8, p, None, p, 8, None, 0, None]
+    for i in (1, 2, 3, 5, 7):                                             # a null operand
+        assert L.wqaa_block_matmul(*(ok[:i] + [None] + ok[i + 1:])) == wlib.ERR_BAD_DESC
+    assert L.wqaa_block_matmul(*(ok[:4] + [7] + ok[5:])) == wlib.ERR_BAD_DESC          # scale rows overlap
+    assert L.wqaa_block_matmul(*(ok[:1] + [p + 8] + ok[2:])) == wlib.ERR_BAD_DESC      # A off its alignment
+    assert L.wqaa_block_matmul(*(ok[:8] + [-1] + ok[9:])) == wlib.ERR_BAD_DESC
+    assert L.wqaa_block_matmul(*(ok[:8] + [0] + ok[9:])) == wlib.OK                    # no rows: nothing to do, no device asked for
+    d.with_bias = 1
+    assert L.wqaa_block_matmul(*ok) == wlib.ERR_BAD_DESC
+
+
+def test_plans_cover_every_row_count():
+    op = bitblas.BlockScaledMatmul(bitblas.BlockScaledMatmulConfig(N=4096, K=4096))
+    for m in (1, 2, 16, 17, 32, 33, 64, 65, 128, 129, 333, 1024, 4096, 100000):
+        plan = op.plan(m)
+        assert plan["grid"] > 0 and plan["block_k"] == 128 and plan["name"].startswith("block_matmul")
+        assert (op.workspace_bytes(m) > 0) == (plan["split_k"] > 1)
+
+
+def _quant(**kw):
+    q = bs.BlockQuant()
+    q.struct_size = ctypes.sizeof(bs.BlockQuant)
+    q.x_dtype, q.q_dtype, q.rows, q.K, q.x_ld, q.gate_ld, q.s_ld = wlib.F16, wlib.E4M3, 4, 256, 256, 256, 4
+    q.X = q.Q = q.S = 4096
+    for k, v in kw.items():
+        setattr(q, k, v)
+    return q
+
+
+@pytest.mark.parametrize("kw", [dict(struct_size=8), dict(rows=-1), dict(K=0), dict(X=None), dict(Q=None), dict(S=None), dict(x_ld=255),
+                                dict(gate=4096, gate_ld=8), dict(s_ld=3)])
+def test_quantizer_refusals(kw):
+    assert bs._library().wqaa_block_quantize(ctypes.byref(_quant(**kw)), None) == wlib.ERR_BAD_DESC
+    assert bs._library().wqaa_block_quantize(ctypes.byref(_quant(rows=0)), None) == wlib.OK
+
+
+def _norm(**kw):
+    n = bs.ResidualNormArgs()
+    n.struct_size = ctypes.sizeof(bs.ResidualNormArgs)
+    n.x_dtype, n.stream_dtype, n.weight_dtype, n.q_dtype = wlib.F16, wlib.F16, wlib.F16, -1
+    n.rows, n.D, n.x_ld, n.residual_ld, n.gate_rows = 4, 256, 256, 256, 1
+    n.x = n.weight = n.Y = 4096
+    for k, v in kw.items():
+        setattr(n, k, v)
+    return n
+
+
+@pytest.mark.parametrize("kw", [dict(struct_size=8), dict(rows=-1), dict(D=0), dict(x=None), dict(Y=None), dict(weight=None), dict(x_ld=100),
+                                dict(residual=4096, residual_ld=0), dict(gate=4096, gate_rows=0), dict(gate=4096, gate_ld=-1),
+                                dict(q_dtype=wlib.E4M3), dict(q_dtype=wlib.E4M3, S=4096, s_ld=3)])
+def test_norm_refusals(kw):
+    assert bs._library().wqaa_residual_norm(ctypes.byref(_norm(**kw)), None) == wlib.ERR_BAD_DESC
+    assert bs._library().wqaa_residual_norm(ctypes.byref(_norm(rows=0)), None) == wlib.OK
+
+
+def test_host_tensors_are_refused():
+    x = torch.randn(2, 128, dtype=torch.float16)
+    op = bitblas.BlockScaledMatmul(bitblas.BlockScaledMatmulConfig(N=128, K=128))
+    q, s = x.to(torch.float8_e4m3fn), torch.ones(2, 1)
+    for call in (lambda: bitblas.quantize_blocks(x), lambda: bitblas.residual_norm(x, x, x[0]), lambda: op(q, q, s, s)):
+        with pytest.raises(RuntimeError, match="GPU"):
+            call()
+
+
+def test_row_layouts():
+    t = torch.arange(4 * 6 * 10).view(4, 6, 10)
+    for view, ld in ((t, 10), (t[:, :, 2:7], 10), (t[1:3, :, :4], 10), (t.view(24, 10)[::2], 20), (t[0], 10), (t[:, 2], 60)):
+        got, d = bs._rows(view)
+        assert d == ld and got.data_ptr() == view.data_ptr()
+        k = view.shape[-1]
+        flat = torch.as_strided(got, (view.numel() // k, k), (d, 1))
+        assert torch.equal(flat, view.reshape(-1, k))
+    for view in (t[:, ::2], t.transpose(0, 1), t[..., ::2], t[0].t(), t[:1].expand(4, 6, 10)):
+        got, d = bs._rows(view)
+        k = view.shape[-1]
+        assert torch.equal(torch.as_strided(got, (view.numel() // k, k), (d, 1)), view.reshape(-1, k))
+
+
+@pytest.mark.parametrize("shape", [(7,), (1, 7), (4, 1, 7), (4, 3, 7), (1, 3, 7), (3, 7), (4, 3, 1), (1,), (1, 1, 7), ()])
+def test_gate_layouts(shape):
+    x = torch.zeros(4, 3, 7)
+    gate = torch.arange(float(max(1, torch.Size(shape).numel()))).reshape(shape)
+    g, ld, share = bs._gate_rows(gate, x)
+    want = gate.expand(4, 3, 7).reshape(12, 7)
+    flat = torch.stack([torch.as_strided(g, (7,), (1,), g.storage_offset() + r // share * ld) for r in range(12)])
+    assert torch.equal(flat, want)
+
+
+def test_gate_of_another_shape_is_refused():
+    with pytest.raises(ValueError):
+        bs._gate_rows(torch.zeros(5, 7), torch.zeros(4, 3, 7))
+
+
+def test_scale_layouts():
+    made = bs._new_scales((2, 3), 6, 5, "cpu")
+    assert made.shape == (2, 3, 5)
+    flat, ld = bs._scale_rows(made, 6, 5)
+    assert flat.data_ptr() == made.data_ptr() and ld == 6 and flat.stride(0) == 1
+    plain = torch.arange(30.0).view(6, 5)
+    flat, ld = bs._scale_rows(plain, 6, 5)
+    assert ld == 6 and torch.equal(flat, plain) and flat.stride() == (1, 6)
+    one, ld = bs._scale_rows(torch.arange(5.0).view(1, 5), 1, 5)
+    assert ld == 1 and one.shape == (1, 5)
+    wide = torch.empty(5, 9).t()[:6]                                     # rows of a block side by side, blocks further apart
+    assert bs._scale_rows(wide, 6, 5)[1] == 9
