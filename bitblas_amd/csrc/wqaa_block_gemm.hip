@@ -1,5 +1,6 @@
 // wqaa_block_gemm.hip - the block-scaled 8-bit product: which member a call takes, and its launch.
 #include "wqaa_block_gemm_kernel.h"
+#include "wqaa_block_pp_kernel.h"
 
 namespace wqaa {
 
@@ -7,7 +8,7 @@ namespace {
 
 struct Choice {
   int stream_waves;      // > 0: the streaming member with this many waves
-  int bm;                // tile member: activation rows of a tile
+  int bm;                // tile members: activation rows of a tile (256: the ping-pong member, whose tiles are 256 weight rows wide)
   int tiles_m, tiles_n, split, split_len;
 };
 
@@ -18,6 +19,15 @@ Choice choose(const wqaa_block_desc& d, int m) {
     c.stream_waves = kb >= 16 ? 8 : 4;
     c.tiles_m = 1, c.tiles_n = (d.N + 15) / 16, c.split = 1, c.split_len = kb;
     return c;
+  }
+  {
+    const long tiles = (long)((m + 255) / 256) * ((d.N + 255) / 256);
+    if (m > 128 && tiles >= 192) {
+      c.bm = 256;
+      c.tiles_m = (m + 255) / 256, c.tiles_n = (d.N + 255) / 256;
+      c.split = 1, c.split_len = kb;
+      return c;
+    }
   }
   c.bm = m <= 32 ? 32 : m <= 64 ? 64 : 128;
   c.tiles_m = (m + c.bm - 1) / c.bm;
@@ -40,8 +50,14 @@ template <class P>
 void tile_go(const BlockGemmArgs& a, hipStream_t s) {
   wq_block_tile_kernel<P><<<dim3(a.tiles_m * a.tiles_n * a.split), dim3(P::THREADS), P::LDS, s>>>(a);
 }
+template <int WF, int AF, bool TAIL>
+void pp_attr() {
+  (void)hipFuncSetAttribute(reinterpret_cast<const void*>(wq_block_pp_kernel<WF, AF, TAIL>), hipFuncAttributeMaxDynamicSharedMemorySize, BlockPP::LDS);
+}
 template <int WF, int AF>
 void init_pair() {
+  pp_attr<WF, AF, false>();
+  pp_attr<WF, AF, true>();
   tile_attr<BlockTile<WF, AF, 32, 3>>();
   tile_attr<BlockTile<WF, AF, 64, 3>>();
   tile_attr<BlockTile<WF, AF, 128, 4>>();
@@ -52,7 +68,9 @@ void launch_pair(const Choice& c, const BlockGemmArgs& a, hipStream_t s) {
   else if (c.stream_waves == 4) wq_block_stream_kernel<WF, AF, 4><<<dim3(a.tiles_n), dim3(256), 0, s>>>(a);
   else if (c.bm == 32) tile_go<BlockTile<WF, AF, 32, 3>>(a, s);
   else if (c.bm == 64) tile_go<BlockTile<WF, AF, 64, 3>>(a, s);
-  else tile_go<BlockTile<WF, AF, 128, 4>>(a, s);
+  else if (c.bm == 128) tile_go<BlockTile<WF, AF, 128, 4>>(a, s);
+  else if (a.K % kBlock) wq_block_pp_kernel<WF, AF, true><<<dim3(a.tiles_m * a.tiles_n), dim3(BlockPP::THREADS), BlockPP::LDS, s>>>(a);
+  else wq_block_pp_kernel<WF, AF, false><<<dim3(a.tiles_m * a.tiles_n), dim3(BlockPP::THREADS), BlockPP::LDS, s>>>(a);
 }
 
 }  // namespace
@@ -75,13 +93,13 @@ int block_gemm_plan(const wqaa_block_desc& d, int m, wqaa_plan* plan) {
   memset(plan, 0, sizeof(*plan));
   plan->kernel_family = 2;
   plan->block_m = c.stream_waves ? 16 : c.bm;
-  plan->block_n = c.stream_waves ? 16 : 128;
+  plan->block_n = c.stream_waves ? 16 : c.bm == 256 ? 256 : 128;
   plan->block_k = kBlock;
-  plan->threads = c.stream_waves ? c.stream_waves * 64 : 256;
+  plan->threads = c.stream_waves ? c.stream_waves * 64 : c.bm == 256 ? BlockPP::THREADS : 256;
   plan->grid = c.tiles_m * c.tiles_n * c.split;
   plan->split_k = c.split;
   snprintf(plan->name, sizeof(plan->name), "block_matmul_m%dn%dk%d_%sx%s_%s%dx%d%s", m, d.N, d.K, short_dtype(d.a_dtype), short_dtype(d.w_dtype),
-           c.stream_waves ? "stream" : "tile", plan->block_m, plan->block_n, c.split > 1 ? "_split" : "");
+           c.stream_waves ? "stream" : c.bm == 256 ? "pp" : "tile", plan->block_m, plan->block_n, c.split > 1 ? "_split" : "");
   return WQAA_OK;
 }
 

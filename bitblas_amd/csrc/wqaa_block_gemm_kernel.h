@@ -25,7 +25,7 @@ template <int WF, int AF>
 __device__ __forceinline__ bf32x4 block_mfma(const bi32x4 (&w)[2], const bi32x4 (&a)[2]) {
   const bi32x8 wv = {w[0][0], w[0][1], w[0][2], w[0][3], w[1][0], w[1][1], w[1][2], w[1][3]};
   const bi32x8 av = {a[0][0], a[0][1], a[0][2], a[0][3], a[1][0], a[1][1], a[1][2], a[1][3]};
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wv, av, bf32x4{0.f, 0.f, 0.f, 0.f}, WF, AF, 0, 0x7F7F7F7F, 0, 0x7F7F7F7F);
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wv, av, bf32x4{0.f, 0.f, 0.f, 0.f}, WF, AF, 0, 0, 0, 0);   // (scales of 0: the form without scales)
 }
 
 __device__ __forceinline__ uint16_t block_bf16(float f) {
