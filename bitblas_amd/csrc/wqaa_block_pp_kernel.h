@@ -34,7 +34,7 @@ struct BlockPP {
 };
 
 // v: lane (r, q) holds row q * 16 + r  ->  out[j]: every lane (r, .) holds row j * 16 + r
-__device__ __forceinline__ void block_spread4(float v, float (&out)[4]) {
+__device__ __forceinline__ void block_spread4(float v, float* out) {
   const uint32_t u = __builtin_bit_cast(uint32_t, v);
   const auto h = __builtin_amdgcn_permlane32_swap(u, u, false, false);          // rows 0, 1 twice | rows 2, 3 twice
   const auto a = __builtin_amdgcn_permlane16_swap(h[0], h[0], false, false);
@@ -118,6 +118,7 @@ __global__ void __launch_bounds__(BlockPP::THREADS) wq_block_pp_kernel(const Blo
   block_wait_vm<8>();
   WQ_BLOCK_BARRIER();
   if (grp == 1) WQ_BLOCK_BARRIER();
+  block_spread4(raw[0] * sw, s);
 
   bf32x4 d[3] = {};
   auto scaled = [&](auto PH, int j) {                               // result j of segment PH onto its sums
@@ -147,18 +148,11 @@ __global__ void __launch_bounds__(BlockPP::THREADS) wq_block_pp_kernel(const Blo
       af[f][0] = *reinterpret_cast<const bi32x4*>(as + f * 2048 + rd0);
       af[f][1] = *reinterpret_cast<const bi32x4*>(as + f * 2048 + rd1);
     }
-    finish(std::integral_constant<int, 1 - p>{});                        // (block 0, segment 0: the results are zero)
+    const int dslot = slot + 2 >= 3 ? slot - 1 : slot + 2;
+    const float hi = raw[1] * sw;                                         // (segment 0: this block's rows 64 ... 127; segment 1: not used)
     if constexpr (p == 0) {
-      float lo[4], hi[4];
-      block_spread4(raw[0] * sw, lo);
-      block_spread4(raw[1] * sw, hi);
-#pragma unroll
-      for (int f = 0; f < 4; ++f) s[f] = lo[f], s[4 + f] = hi[f];
       fetch_scales(t + 1);
       sw = swp[min(t + 1, nt - 1)];
-    }
-    const int dslot = slot + 2 >= 3 ? slot - 1 : slot + 2;
-    if constexpr (p == 0) {
       dma_a(t + 2, dslot, 0);
       dma_a(t + 2, dslot, 1);
     } else {
@@ -167,6 +161,13 @@ __global__ void __launch_bounds__(BlockPP::THREADS) wq_block_pp_kernel(const Blo
 #pragma unroll
       for (int j = 0; j < 4; ++j) dma_w(t + 2, t & 1, j);
     }
+    // vector work in the shadow of the operand reads: the last two results of the segment before, then the scales whose fragments
+    // are through - the second half's in segment 0, the next block's first half's in segment 1
+    __builtin_amdgcn_sched_barrier(0);
+    finish(std::integral_constant<int, 1 - p>{});                        // (block 0, segment 0: the results are zero)
+    if constexpr (p == 0) block_spread4(hi, s + 4);
+    else block_spread4(raw[0] * sw, s);
+    __builtin_amdgcn_sched_barrier(0);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     if constexpr (p == 1) block_wait_vm<8>();
     WQ_BLOCK_BARRIER();
