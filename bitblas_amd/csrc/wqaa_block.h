@@ -13,11 +13,12 @@ struct BlockGemmArgs {
   const float* sw;                           // scale of (tile t, block b) at sw[t * KB + b]
   const void* bias;                          // (N,) of the output type, or null
   void* C;                                   // (M, N)
-  float* ws;                                 // split K: (split, M, N) partial sums
+  float* ws;                                 // partial tiles of the K slices: (tile, slice, BM, 128)
   long sa_ld;
   int M, N, K, KB;                           // KB = ceil(K / 128)
   int out_dtype;                             // wqaa_dtype
   int tiles_m, tiles_n;
+  int whole;                                 // tiles with a workgroup of their own; each tile behind them is shared by `split`
   int split, split_len;                      // k-blocks [z * split_len, min(KB, (z + 1) * split_len)) for slice z
   int group_m;                               // M-tiles that share an N-tile back to back
 };

@@ -9,7 +9,9 @@ namespace {
 struct Choice {
   int stream_waves;      // > 0: the streaming member with this many waves
   int bm;                // tile members: activation rows of a tile (256: the ping-pong member, whose tiles are 256 weight rows wide)
-  int tiles_m, tiles_n, split, split_len;
+  int tiles_m, tiles_n, whole, split, split_len;   // workgroups: whole + (tiles_m tiles_n - whole) split
+  long tail() const { return (long)tiles_m * tiles_n - whole; }
+  long grid() const { return whole + tail() * split; }
 };
 
 Choice choose(const wqaa_block_desc& d, int m) {
@@ -17,7 +19,7 @@ Choice choose(const wqaa_block_desc& d, int m) {
   const int kb = (d.K + kBlock - 1) / kBlock;
   if (m <= 16) {
     c.stream_waves = kb >= 16 ? 8 : 4;
-    c.tiles_m = 1, c.tiles_n = (d.N + 15) / 16, c.split = 1, c.split_len = kb;
+    c.tiles_m = 1, c.tiles_n = (d.N + 15) / 16, c.whole = c.tiles_n, c.split = 1, c.split_len = kb;
     return c;
   }
   {
@@ -25,18 +27,21 @@ Choice choose(const wqaa_block_desc& d, int m) {
     if (m > 128 && tiles >= 192) {
       c.bm = 256;
       c.tiles_m = (m + 255) / 256, c.tiles_n = (d.N + 255) / 256;
-      c.split = 1, c.split_len = kb;
+      c.whole = (int)tiles, c.split = 1, c.split_len = kb;
       return c;
     }
   }
   c.bm = m <= 32 ? 32 : m <= 64 ? 64 : 128;
   c.tiles_m = (m + c.bm - 1) / c.bm;
   c.tiles_n = (d.N + kBlock - 1) / kBlock;
-  // fewer tiles than CUs: K in slices of at least 4 blocks, so that the slices fill the chip once
+  // whole rounds of the chip (a tile per CU) take tiles with a workgroup of their own; what is left over is cut along K, in slices of
+  // at least 2 blocks, so that it fills the chip once and not a last round of whole tiles
   const long tiles = (long)c.tiles_m * c.tiles_n;
-  long split = tiles >= 256 ? 1 : 256 / tiles;
-  if (split > kb / 4) split = kb / 4;
-  if (split < 1) split = 1;
+  long rest = tiles % 256;
+  long split = rest ? 512 / rest : 1;
+  if (split > kb / 2) split = kb / 2;
+  if (split < 2 || tiles > 4096) split = 1, rest = 0;
+  c.whole = (int)(tiles - rest);
   c.split_len = (int)((kb + split - 1) / split);
   c.split = (kb + c.split_len - 1) / c.split_len;
   return c;
@@ -47,8 +52,8 @@ void tile_attr() {
   (void)hipFuncSetAttribute(reinterpret_cast<const void*>(wq_block_tile_kernel<P>), hipFuncAttributeMaxDynamicSharedMemorySize, P::LDS);
 }
 template <class P>
-void tile_go(const BlockGemmArgs& a, hipStream_t s) {
-  wq_block_tile_kernel<P><<<dim3(a.tiles_m * a.tiles_n * a.split), dim3(P::THREADS), P::LDS, s>>>(a);
+void tile_go(const Choice& c, const BlockGemmArgs& a, hipStream_t s) {
+  wq_block_tile_kernel<P><<<dim3((unsigned)c.grid()), dim3(P::THREADS), P::LDS, s>>>(a);
 }
 template <int WF, int AF, bool TAIL>
 void pp_attr() {
@@ -60,15 +65,15 @@ void init_pair() {
   pp_attr<WF, AF, true>();
   tile_attr<BlockTile<WF, AF, 32, 3>>();
   tile_attr<BlockTile<WF, AF, 64, 3>>();
-  tile_attr<BlockTile<WF, AF, 128, 4>>();
+  tile_attr<BlockTile<WF, AF, 128, 2>>();
 }
 template <int WF, int AF>
 void launch_pair(const Choice& c, const BlockGemmArgs& a, hipStream_t s) {
   if (c.stream_waves == 8) wq_block_stream_kernel<WF, AF, 8><<<dim3(a.tiles_n), dim3(512), 0, s>>>(a);
   else if (c.stream_waves == 4) wq_block_stream_kernel<WF, AF, 4><<<dim3(a.tiles_n), dim3(256), 0, s>>>(a);
-  else if (c.bm == 32) tile_go<BlockTile<WF, AF, 32, 3>>(a, s);
-  else if (c.bm == 64) tile_go<BlockTile<WF, AF, 64, 3>>(a, s);
-  else if (c.bm == 128) tile_go<BlockTile<WF, AF, 128, 4>>(a, s);
+  else if (c.bm == 32) tile_go<BlockTile<WF, AF, 32, 3>>(c, a, s);
+  else if (c.bm == 64) tile_go<BlockTile<WF, AF, 64, 3>>(c, a, s);
+  else if (c.bm == 128) tile_go<BlockTile<WF, AF, 128, 2>>(c, a, s);
   else if (a.K % kBlock) wq_block_pp_kernel<WF, AF, true><<<dim3(a.tiles_m * a.tiles_n), dim3(BlockPP::THREADS), BlockPP::LDS, s>>>(a);
   else wq_block_pp_kernel<WF, AF, false><<<dim3(a.tiles_m * a.tiles_n), dim3(BlockPP::THREADS), BlockPP::LDS, s>>>(a);
 }
@@ -84,7 +89,7 @@ void block_init() {
 
 size_t block_gemm_workspace_bytes(const wqaa_block_desc& d, int m) {
   const Choice c = choose(d, m);
-  return c.split > 1 ? (size_t)c.split * m * d.N * 4 : 0;
+  return c.split > 1 ? (size_t)c.tail() * c.split * c.bm * kBlock * 4 : 0;
 }
 
 int block_gemm_plan(const wqaa_block_desc& d, int m, wqaa_plan* plan) {
@@ -96,7 +101,7 @@ int block_gemm_plan(const wqaa_block_desc& d, int m, wqaa_plan* plan) {
   plan->block_n = c.stream_waves ? 16 : c.bm == 256 ? 256 : 128;
   plan->block_k = kBlock;
   plan->threads = c.stream_waves ? c.stream_waves * 64 : c.bm == 256 ? BlockPP::THREADS : 256;
-  plan->grid = c.tiles_m * c.tiles_n * c.split;
+  plan->grid = (int)c.grid();
   plan->split_k = c.split;
   snprintf(plan->name, sizeof(plan->name), "block_matmul_m%dn%dk%d_%sx%s_%s%dx%d%s", m, d.N, d.K, short_dtype(d.a_dtype), short_dtype(d.w_dtype),
            c.stream_waves ? "stream" : c.bm == 256 ? "pp" : "tile", plan->block_m, plan->block_n, c.split > 1 ? "_split" : "");
@@ -111,7 +116,7 @@ int block_gemm_launch(const wqaa_block_desc& d, const void* A, const void* W, co
     set_error(WQAA_ERR_BAD_DESC, "block_matmul: m=%d needs %llu bytes of 16-byte aligned workspace", m, (unsigned long long)need);
     return WQAA_ERR_BAD_DESC;
   }
-  if ((long)c.tiles_m * c.tiles_n * c.split > 0x7fffffffl || (int64_t)m * 4 > 0x7fffffff) {
+  if ((long)c.tiles_m * c.tiles_n > 0x3fffffffl || (int64_t)m * 4 > 0x7fffffff) {
     set_error(WQAA_ERR_UNSUPPORTED, "block_matmul: m=%d N=%d is too large", m, d.N);
     return WQAA_ERR_UNSUPPORTED;
   }
@@ -122,14 +127,14 @@ int block_gemm_launch(const wqaa_block_desc& d, const void* A, const void* W, co
   a.C = C, a.ws = reinterpret_cast<float*>(workspace);
   a.M = m, a.N = d.N, a.K = d.K, a.KB = (d.K + kBlock - 1) / kBlock;
   a.out_dtype = d.out_dtype;
-  a.tiles_m = c.tiles_m, a.tiles_n = c.tiles_n, a.split = c.split, a.split_len = c.split_len;
+  a.tiles_m = c.tiles_m, a.tiles_n = c.tiles_n, a.whole = c.whole, a.split = c.split, a.split_len = c.split_len;
   a.group_m = c.tiles_m < 8 ? c.tiles_m : 8;
   const int wf = d.w_dtype == WQAA_E5M2, af = d.a_dtype == WQAA_E5M2;
   if (wf == 0 && af == 0) launch_pair<0, 0>(c, a, stream);
   else if (wf == 0) launch_pair<0, 1>(c, a, stream);
   else if (af == 0) launch_pair<1, 0>(c, a, stream);
   else launch_pair<1, 1>(c, a, stream);
-  if (c.split > 1) wq_block_reduce_kernel<<<dim3((unsigned)(((long)m * d.N + 255) / 256)), dim3(256), 0, stream>>>(a);
+  if (c.split > 1) wq_block_reduce_kernel<<<dim3((unsigned)(c.tail() * (c.bm / 8))), dim3(256), 0, stream>>>(a, c.bm);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) {
     set_error(WQAA_ERR_LAUNCH, "block_matmul: %s", hipGetErrorString(e));

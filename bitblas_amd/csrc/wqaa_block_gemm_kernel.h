@@ -110,7 +110,10 @@ __global__ void __launch_bounds__(WAVES * 64) wq_block_stream_kernel(const Block
 // ---- m > 16: tiles of BM x 128 through LDS ------------------------------------------------------------------------------------------
 // Four waves, S stages of one k-block each, every byte by LDS-DMA.  A stage holds BM activation rows and 128 weight rows of 128 bytes,
 // 16-byte piece g of row r at slot g ^ ((r >> 1) & 7) (the lanes of an operand read then hit every bank twice, which is the rate),
-// and per wave the scales of its own activation rows (64 of them; rows beyond M read as zero).
+// and per wave the scales of its own activation rows (64 of them; rows beyond M read as zero).  Half a CU's LDS at most: two
+// workgroups share a CU, and one's copies and operand reads run under the other's matrix instructions.
+// The grid is `whole` workgroups of one tile each, then `split` workgroups for each of the remaining tiles: those that would start
+// another round of the chip take a K slice each and leave float32 partial tiles for the reduce launch behind this one.
 template <int WF_, int AF_, int BM_, int S_>
 struct BlockTile {
   static constexpr int WF = WF_, AF = AF_, BM = BM_, BN = 128, S = S_, THREADS = 256;
@@ -121,7 +124,7 @@ struct BlockTile {
   static constexpr int AP = BM / 32, WP = BN / 32;                       // DMA pieces (8 rows) of a wave per stage
   static constexpr int PIECES = AP + WP + 1;
   static constexpr int LDS = S * STAGE;
-  static_assert(LDS <= 160 * 1024 && MF * 16 <= 64, "LDS budget; one DMA piece holds a wave's row scales");
+  static_assert(LDS <= 80 * 1024 && MF * 16 <= 64, "two workgroups a CU; one DMA piece holds a wave's row scales");
 };
 
 template <int N>
@@ -129,8 +132,29 @@ __device__ __forceinline__ void block_wait_vm() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 
+#define WQ_BLOCK_BARRIER()                  \
+  do {                                      \
+    asm volatile("" ::: "memory");          \
+    __builtin_amdgcn_sched_barrier(0);      \
+    __builtin_amdgcn_s_barrier();           \
+    __builtin_amdgcn_sched_barrier(0);      \
+    asm volatile("" ::: "memory");          \
+  } while (0)
+
+// tile `blk` of `nblk`: an XCD's workgroups (index modulo 8) walk neighbouring tiles, group_m M-tiles for each N-tile
+__device__ __forceinline__ void block_tile_of(const BlockGemmArgs& a, int blk, int nblk, int& tile_m, int& tile_n) {
+  if ((nblk & 7) == 0) blk = (blk & 7) * (nblk >> 3) + (blk >> 3);
+  const int per_group = a.group_m * a.tiles_n;
+  const int group = blk / per_group;
+  const int first_m = group * a.group_m;
+  const int gsz = min(a.group_m, a.tiles_m - first_m);
+  const int rem = blk - group * per_group;
+  tile_m = first_m + rem % gsz;
+  tile_n = rem / gsz;
+}
+
 template <class P>
-__global__ void __launch_bounds__(P::THREADS) wq_block_tile_kernel(const BlockGemmArgs a) {
+__global__ void __launch_bounds__(P::THREADS, 2) wq_block_tile_kernel(const BlockGemmArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
   typedef __attribute__((address_space(3))) void* lds_t;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
@@ -138,21 +162,17 @@ __global__ void __launch_bounds__(P::THREADS) wq_block_tile_kernel(const BlockGe
   const int r = lane & 15, q = lane >> 4;
   const int wm = wave / P::WN, wn = wave % P::WN;
 
-  // workgroup -> (slice, tile): the workgroups of an XCD (block index modulo 8) walk neighbouring tiles, group_m M-tiles per N-tile
-  int blk = blockIdx.x;
-  const int nblk = gridDim.x;
-  if ((nblk & 7) == 0) blk = (blk & 7) * (nblk >> 3) + (blk >> 3);
-  const int per_slice = a.tiles_m * a.tiles_n;
-  const int slice = blk / per_slice;
-  blk -= slice * per_slice;
-  const int per_group = a.group_m * a.tiles_n;
-  const int group = blk / per_group;
-  const int first_m = group * a.group_m;
-  const int gsz = min(a.group_m, a.tiles_m - first_m);
-  const int rem = blk - group * per_group;
-  const int m0 = (first_m + rem % gsz) * P::BM, n0 = rem / gsz * P::BN;
-
-  const int b_first = slice * a.split_len, b_end = min(a.KB, b_first + a.split_len);
+  int tile_m, tile_n, b_first = 0, b_end = a.KB, piece = -1;
+  if ((int)blockIdx.x < a.whole) {
+    block_tile_of(a, blockIdx.x, a.whole, tile_m, tile_n);
+  } else {
+    piece = blockIdx.x - a.whole;
+    const int t = piece / a.split;
+    b_first = (piece - t * a.split) * a.split_len;
+    b_end = min(a.KB, b_first + a.split_len);
+    block_tile_of(a, a.whole + t, 1, tile_m, tile_n);
+  }
+  const int m0 = tile_m * P::BM, n0 = tile_n * P::BN;
 
   // tile-relative buffers: the range ends with the matrix, so rows beyond it read as zero
   const long a_bytes = (long)min(P::BM, a.M - m0) * a.K, w_bytes = (long)min(P::BN, a.N - n0) * a.K;
@@ -161,8 +181,9 @@ __global__ void __launch_bounds__(P::THREADS) wq_block_tile_kernel(const BlockGe
   const int pr = lane >> 3;                                              // row of a piece
   const int g0 = (lane & 7) ^ ((lane >> 4) & 7), g1 = g0 ^ 4;            // source granule of even / odd pieces
   constexpr uint32_t OUT = 0xC0000000u;                                  // beyond every buffer: reads as zero
+  const uint32_t va = (uint32_t)(wave * (P::BM / 4) + pr) * (uint32_t)a.K, vw = (uint32_t)(wave * (P::BN / 4) + pr) * (uint32_t)a.K;
   const int sm = m0 + wm * (P::MF * 16) + lane;                          // the row whose scale this lane fetches
-  const bool sm_ok = lane < P::MF * 16 && sm < a.M;
+  const uint32_t vs = lane < P::MF * 16 && sm < a.M ? (uint32_t)sm * 4u : OUT;
   const int last = a.KB - 1;
   const int tail = a.K - last * kBlock;                                  // k in the last block
 
@@ -170,22 +191,24 @@ __global__ void __launch_bounds__(P::THREADS) wq_block_tile_kernel(const BlockGe
     const int b = min(b_first + t, b_end - 1);                           // (beyond the slice: the last block again, never used)
     unsigned char* base = smem + slot * P::STAGE;
     const bool cut = b == last;
-    const uint32_t k0 = (cut && g0 * 16 >= tail) ? OUT : (uint32_t)(g0 * 16), k1 = (cut && g1 * 16 >= tail) ? OUT : (uint32_t)(g1 * 16);
+    const bool out0 = cut && g0 * 16 >= tail, out1 = cut && g1 * 16 >= tail;
+    const uint32_t k0 = g0 * 16, k1 = g1 * 16;
 #pragma unroll
     for (int j = 0; j < P::AP; ++j) {
       const int row = wave * (P::BM / 4) + j * 8;
-      const uint32_t k = (row & 8) ? k1 : k0;
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(a_rsrc, (lds_t)(base + row * 128), 16, k == OUT ? OUT : k + (uint32_t)(row + pr) * (uint32_t)a.K, b * kBlock, 0, 0);
+      const bool odd = P::BM == 32 ? (wave & 1) : (j & 1);
+      const uint32_t v = va + (uint32_t)(j * 8) * (uint32_t)a.K + (odd ? k1 : k0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(a_rsrc, (lds_t)(base + row * 128), 16, (odd ? out1 : out0) ? OUT : v, b * kBlock, 0, 0);
     }
 #pragma unroll
     for (int j = 0; j < P::WP; ++j) {
       const int row = wave * (P::BN / 4) + j * 8;
-      const uint32_t k = (row & 8) ? k1 : k0;
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(w_rsrc, (lds_t)(base + P::A_BYTES + row * 128), 16, k == OUT ? OUT : k + (uint32_t)(row + pr) * (uint32_t)a.K, b * kBlock, 0, 0);
+      const uint32_t v = vw + (uint32_t)(j * 8) * (uint32_t)a.K + ((j & 1) ? k1 : k0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(w_rsrc, (lds_t)(base + P::A_BYTES + row * 128), 16, ((j & 1) ? out1 : out0) ? OUT : v, b * kBlock, 0, 0);
     }
     // this wave's row scales of the block, 4 bytes a lane
-    const auto s_rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(a.sa + (long)b * a.sa_ld), 0, 0x7FFFFFFF, 0x00020000);
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(s_rsrc, (lds_t)(base + P::A_BYTES + P::W_BYTES + wave * 256), 4, sm_ok ? (uint32_t)sm * 4u : OUT, 0, 0, 0);
+    const auto s_rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(a.sa + (long)b * a.sa_ld), 0, a.M * 4, 0x00020000);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(s_rsrc, (lds_t)(base + P::A_BYTES + P::W_BYTES + wave * 256), 4, vs, 0, 0, 0);
   };
 
   bf32x4 acc[P::MF][P::NF];
@@ -195,19 +218,20 @@ __global__ void __launch_bounds__(P::THREADS) wq_block_tile_kernel(const BlockGe
     for (int g = 0; g < P::NF; ++g) acc[f][g] = bf32x4{0.f, 0.f, 0.f, 0.f};
   const int swl = (r >> 1) & 7;
   const int rd0 = r * 128 + ((q ^ swl) * 16), rd1 = r * 128 + (((4 + q) ^ swl) * 16);
-  const float* swp = a.sw + (long)(n0 / kBlock) * a.KB + b_first;
+  const auto* swp = (const __attribute__((address_space(4))) float*)(a.sw + (long)tile_n * a.KB + b_first);
 
   const int nt = b_end - b_first;
 #pragma unroll
   for (int t = 0; t < P::S - 1; ++t) stage(t, t);
   int slot = 0, fill = P::S - 1;
   for (int t = 0; t < nt; ++t) {
+    const float sw = swp[t];
     block_wait_vm<(P::S - 2) * P::PIECES>();      // this wave's pieces of block t have landed (one kind of load in flight: in order)
-    __syncthreads();                              // everyone's have, and everyone is done with block t - 1, whose slot is filled next
+    WQ_BLOCK_BARRIER();                           // everyone's have, and everyone is done with block t - 1, whose slot is filled next
     stage(t + P::S - 1, fill);
     const unsigned char* base = smem + slot * P::STAGE;
-    const float sw = swp[t];
-    bi32x4 w[P::NF][2];
+    bi32x4 w[P::NF][2], x[P::MF][2];
+    float s[P::MF];
 #pragma unroll
     for (int g = 0; g < P::NF; ++g) {
       const unsigned char* p = base + P::A_BYTES + (wn * P::NF + g) * 2048;
@@ -217,15 +241,22 @@ __global__ void __launch_bounds__(P::THREADS) wq_block_tile_kernel(const BlockGe
 #pragma unroll
     for (int f = 0; f < P::MF; ++f) {
       const unsigned char* p = base + (wm * P::MF + f) * 2048;
-      const bi32x4 x[2] = {*reinterpret_cast<const bi32x4*>(p + rd0), *reinterpret_cast<const bi32x4*>(p + rd1)};
-      const float s = reinterpret_cast<const float*>(base + P::A_BYTES + P::W_BYTES + wave * 256)[f * 16 + r] * sw;
+      x[f][0] = *reinterpret_cast<const bi32x4*>(p + rd0);
+      x[f][1] = *reinterpret_cast<const bi32x4*>(p + rd1);
+      s[f] = reinterpret_cast<const float*>(base + P::A_BYTES + P::W_BYTES + wave * 256)[f * 16 + r] * sw;
+    }
+    bf32x4 d[3];
 #pragma unroll
-      for (int g = 0; g < P::NF; ++g) {
-        const bf32x4 d = block_mfma<P::WF, P::AF>(w[g], x);
+    for (int i = 0; i < P::MF * P::NF + 2; ++i) {  // result i's fmas two matrix instructions behind it
+      if (i < P::MF * P::NF) d[i % 3] = block_mfma<P::WF, P::AF>(w[i % P::NF], x[i / P::NF]);
+      __builtin_amdgcn_sched_barrier(0);
+      if (i >= 2) {
+        const int j = i - 2;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) acc[f][g][i] = __builtin_fmaf(d[i], s, acc[f][g][i]);
+        for (int e = 0; e < 4; ++e) acc[j / P::NF][j % P::NF][e] = __builtin_fmaf(d[j % 3][e], s[j / P::NF], acc[j / P::NF][j % P::NF][e]);
       }
     }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // (every operand read has long been used: nothing to wait for)
     slot = slot + 1 == P::S ? 0 : slot + 1;
     fill = fill + 1 == P::S ? 0 : fill + 1;
   }
@@ -233,19 +264,16 @@ __global__ void __launch_bounds__(P::THREADS) wq_block_tile_kernel(const BlockGe
 
 #pragma unroll
   for (int f = 0; f < P::MF; ++f) {
-    const int m = m0 + (wm * P::MF + f) * 16 + r;
+    const int ml = (wm * P::MF + f) * 16 + r, m = m0 + ml;
 #pragma unroll
     for (int g = 0; g < P::NF; ++g) {
-      const int n = n0 + (wn * P::NF + g) * 16 + q * 4;
-      if (m >= a.M || n >= a.N) continue;
-      const int cnt = min(4, a.N - n);
-      if (a.split > 1) {
-        float* o = a.ws + ((long)slice * a.M + m) * a.N + n;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (i < cnt) o[i] = acc[f][g][i];
+      const int nl = (wn * P::NF + g) * 16 + q * 4, n = n0 + nl;
+      if (piece >= 0) {                           // a slice: the whole tile, rows and columns beyond the matrix included
+        *reinterpret_cast<bf32x4*>(a.ws + ((long)piece * P::BM + ml) * P::BN + nl) = acc[f][g];
         continue;
       }
+      if (m >= a.M || n >= a.N) continue;
+      const int cnt = min(4, a.N - n);
       float v[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) v[i] = acc[f][g][i] + (a.bias && i < cnt ? block_bias(a.bias, a.out_dtype, n + i) : 0.f);
@@ -265,15 +293,20 @@ __global__ void __launch_bounds__(P::THREADS) wq_block_tile_kernel(const BlockGe
 #endif
 }
 
-// partial sums of the K slices, in slice order
-__global__ void __launch_bounds__(256) wq_block_reduce_kernel(const BlockGemmArgs a) {
-  const long total = (long)a.M * a.N;
-  const long i = (long)blockIdx.x * 256 + threadIdx.x;
-  if (i >= total) return;
-  float v = 0.f;
-  for (int z = 0; z < a.split; ++z) v += a.ws[z * total + i];
-  if (a.bias) v += block_bias(a.bias, a.out_dtype, (int)(i % a.N));
-  block_store1(a.C, a.out_dtype, i, v);
+// partial tiles of the K slices, in slice order: a workgroup takes 256 x 4 elements of a tile (tile rows of 128, so 8 rows)
+__global__ void __launch_bounds__(256) wq_block_reduce_kernel(const BlockGemmArgs a, int bm) {
+  const int per_tile = bm / 8;
+  const int t = blockIdx.x / per_tile, part = blockIdx.x % per_tile;
+  int tile_m, tile_n;
+  block_tile_of(a, a.whole + t, 1, tile_m, tile_n);
+  const int ml = part * 8 + (threadIdx.x >> 5), nl = (threadIdx.x & 31) * 4;
+  const int m = tile_m * bm + ml, n = tile_n * kBlock + nl;
+  if (m >= a.M || n >= a.N) return;
+  const float* p = a.ws + ((long)t * a.split * bm + ml) * kBlock + nl;
+  bf32x4 v = {0.f, 0.f, 0.f, 0.f};
+  for (int z = 0; z < a.split; ++z) v += *reinterpret_cast<const bf32x4*>(p + (long)z * bm * kBlock);
+  const int cnt = min(4, a.N - n);
+  for (int i = 0; i < cnt; ++i) block_store1(a.C, a.out_dtype, (long)m * a.N + n + i, v[i] + (a.bias ? block_bias(a.bias, a.out_dtype, n + i) : 0.f));
 }
 
 }  // namespace wqaa

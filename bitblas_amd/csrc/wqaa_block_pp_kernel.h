@@ -18,15 +18,6 @@
 
 namespace wqaa {
 
-#define WQ_BLOCK_BARRIER()                  \
-  do {                                      \
-    asm volatile("" ::: "memory");          \
-    __builtin_amdgcn_sched_barrier(0);      \
-    __builtin_amdgcn_s_barrier();           \
-    __builtin_amdgcn_sched_barrier(0);      \
-    asm volatile("" ::: "memory");          \
-  } while (0)
-
 struct BlockPP {
   static constexpr int BM = 256, BN = 256, THREADS = 512;
   static constexpr int SLOT = 256 * 128, W_OFF = 3 * SLOT, LDS = 5 * SLOT;
@@ -56,15 +47,9 @@ __global__ void __launch_bounds__(BlockPP::THREADS) wq_block_pp_kernel(const Blo
   const int grp = wave >> 2, nq = wave & 3;
   const int r = lane & 15, q = lane >> 4;
 
-  int blk = blockIdx.x;
-  const int nblk = gridDim.x;
-  if ((nblk & 7) == 0) blk = (blk & 7) * (nblk >> 3) + (blk >> 3);      // an XCD's workgroups walk neighbouring tiles
-  const int per_group = a.group_m * a.tiles_n;
-  const int group = blk / per_group;
-  const int first_m = group * a.group_m;
-  const int gsz = min(a.group_m, a.tiles_m - first_m);
-  const int rem = blk - group * per_group;
-  const int m0 = (first_m + rem % gsz) * P::BM, n0 = rem / gsz * P::BN;
+  int tile_m, tile_n;
+  block_tile_of(a, blockIdx.x, gridDim.x, tile_m, tile_n);
+  const int m0 = tile_m * P::BM, n0 = tile_n * P::BN;
   const int nt = a.KB;
 
   const long a_bytes = (long)min(P::BM, a.M - m0) * a.K, w_bytes = (long)min(P::BN, a.N - n0) * a.K;
