@@ -33,6 +33,10 @@ _CODE = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16, torch.float32: _lib
          torch.float8_e5m2: _lib.E5M2}
 
 
+_FP8_TYPE = {"e4m3_float8": torch.float8_e4m3fn, "e5m2_float8": torch.float8_e5m2}
+_FLOATS = (torch.float16, torch.bfloat16, torch.float32)
+
+
 def _blocks(n: int) -> int:
     return -(-n // BLOCK)
 
@@ -60,6 +64,7 @@ class ResidualNormArgs(ctypes.Structure):
                 ("Y", ctypes.c_void_p), ("S", ctypes.c_void_p)]
 
 
+_QUANT_BYTES, _NORM_BYTES = ctypes.sizeof(BlockQuant), ctypes.sizeof(ResidualNormArgs)
 _bound = None
 
 
@@ -84,26 +89,21 @@ def _library():
 
 
 def _refuse_grad(what: str, *tensors) -> None:
-    if torch.is_grad_enabled():
-        for t in tensors:
-            if t is not None and t.requires_grad:
-                raise RuntimeError(f"{what} has no backward pass: call it under torch.no_grad(), or detach its inputs")
+    if any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError(f"{what} has no backward pass: call it under torch.no_grad(), or detach its inputs")
 
 
-def _on(what: str, device, *tensors) -> None:
-    for name, t in tensors:
-        if t is not None and t.device != device:
-            raise ValueError(f"{what}: {name} is on {t.device}, the call's input on {device}")
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def _rows(t: torch.Tensor) -> Tuple[torch.Tensor, int]:
     """`t` with its leading dimensions as rows a fixed distance apart: (tensor, distance in elements).  A tensor whose rows are
     not laid out like that is copied."""
     k = t.shape[-1]
-    if t.dim() == 2 and t.stride(1) == 1 and t.stride(0) >= k:
-        return t, t.stride(0)
     if t.is_contiguous():
         return t, k
+    if t.dim() == 2 and t.stride(1) == 1 and t.stride(0) >= k:
+        return t, t.stride(0)
     if t.dim() >= 2 and t.stride(-1) == 1:
         ld = t.stride(-2)
         step = ld
@@ -128,10 +128,32 @@ def _scale_rows(scale: torch.Tensor, m: int, kb: int) -> Tuple[torch.Tensor, int
     return scale, m
 
 
+def _scale_strides(lead: Sequence[int], m: int) -> Tuple[int, ...]:
+    """strides of (*lead, blocks) scales over (blocks, m) storage"""
+    if len(lead) == 1:
+        return (1, m)
+    strides = [m]
+    step = 1
+    for size in reversed(lead):
+        strides.insert(0, step)
+        step *= size
+    return tuple(strides)
+
+
 def _new_scales(lead: Sequence[int], m: int, kb: int, device) -> torch.Tensor:
     """(*lead, kb) float32 scales over (kb, m) storage"""
-    s = torch.empty((kb, m), dtype=torch.float32, device=device)
-    return s.t() if len(lead) == 1 else s.view(kb, *lead).movedim(0, -1)
+    return torch.empty_strided((*lead, kb), _scale_strides(lead, m), dtype=torch.float32, device=device)
+
+
+def _scale_ld(scale: torch.Tensor, lead: Sequence[int], m: int, kb: int) -> int:
+    """distance of two blocks in scales the kernels write"""
+    strides = scale.stride()
+    if strides == _scale_strides(lead, m):
+        return m
+    flat, ld = _scale_rows(scale, m, kb)
+    if flat.data_ptr() != scale.data_ptr():
+        raise ValueError("output scales have the rows of a block side by side, as quantize_blocks returns them")
+    return ld
 
 
 @dataclass(frozen=True)
@@ -176,6 +198,8 @@ class BlockScaledMatmul(Operator):
         self._kb, self._nb = _blocks(self.K), _blocks(self.N)
         self._a, self._w, self._out = torch_dtype(config.A_dtype), torch_dtype(config.W_dtype), torch_dtype(config.out_dtype)
         self.torch_output_dtype = self._out
+        self._w_shape, self._sw_shape, self._bias_shape = torch.Size((self.N, self.K)), torch.Size((self._nb, self._kb)), torch.Size((self.N,))
+        self._with_bias = bool(config.with_bias)
         d = BlockDesc()
         d.struct_size = ctypes.sizeof(BlockDesc)
         d.N, d.K = self.N, self.K
@@ -198,47 +222,82 @@ class BlockScaledMatmul(Operator):
             need = self._need[m] = int(_library().wqaa_block_workspace_bytes(self._ref, int(m)))
         return need
 
-    def forward(self, A, W, scale_a, scale_w, bias=None, output=None):
-        N, K, kb = self.N, self.K, self._kb
-        device = A.device
+    def _refuse(self, A, W, scale_a, scale_w, bias, output):
+        """what `forward` found wrong, in words"""
+        N, K, kb, device, lead = self.N, self.K, self._kb, A.device, tuple(A.shape[:-1])
         if device.type != "cuda":
             raise RuntimeError("BlockScaledMatmul runs on the GPU only")
-        shape = A.shape
-        if A.dtype != self._a or not shape or shape[-1] != K:
-            raise ValueError(f"A is (..., {K}) in {self._a}: got {tuple(shape)} in {A.dtype}")
+        if A.dtype != self._a or A.dim() == 0 or A.shape[-1] != K:
+            raise ValueError(f"A is (..., {K}) in {self._a}: got {tuple(A.shape)} in {A.dtype}")
         if W.dtype != self._w or W.shape != (N, K) or not W.is_contiguous():
             raise ValueError(f"W is a contiguous ({N}, {K}) tensor in {self._w}: got {tuple(W.shape)} in {W.dtype}")
-        lead = shape[:-1]
         if scale_a.dtype != torch.float32 or scale_a.shape != lead + (kb,):
-            raise ValueError(f"scale_a is {tuple(lead) + (kb,)} in float32: got {tuple(scale_a.shape)} in {scale_a.dtype}")
+            raise ValueError(f"scale_a is {lead + (kb,)} in float32: got {tuple(scale_a.shape)} in {scale_a.dtype}")
         if scale_w.dtype != torch.float32 or scale_w.shape != (self._nb, kb) or not scale_w.is_contiguous():
             raise ValueError(f"scale_w is a contiguous ({self._nb}, {kb}) tensor in float32: got {tuple(scale_w.shape)} in {scale_w.dtype}")
         if W.device != device or scale_a.device != device or scale_w.device != device:
             raise ValueError(f"W and the scales must be on A's device ({device})")
+        if W.data_ptr() & 15:
+            raise ValueError("W must be aligned to 16 bytes")
         if (bias is not None) != self.config.with_bias:
             raise ValueError("the bias goes with with_bias, and only with it")
         if bias is not None and (bias.dtype != self._out or bias.shape != (N,) or not bias.is_contiguous() or bias.device != device):
             raise ValueError(f"bias is a contiguous ({N},) tensor in {self._out} on A's device")
-        _refuse_grad("BlockScaledMatmul", scale_a, scale_w, bias)
-        m = A.numel() // K
-        if not A.is_contiguous() or A.data_ptr() & 15:
-            A = A.contiguous() if not A.is_contiguous() else A.clone()
-        if W.data_ptr() & 15:
-            raise ValueError("W must be aligned to 16 bytes")
+        raise ValueError(f"output is a contiguous {lead + (N,)} tensor in {self._out} on A's device")
+
+    def forward(self, A, W, scale_a, scale_w, bias=None, output=None):
+        # (one chain of cheap tests: a decode step's call is as long as its host code)
+        N, K, kb = self.N, self.K, self._kb
+        dev = A.get_device()
+        shape = A.shape
+        lead = shape[:-1]
+        if (dev < 0 or A.dtype is not self._a or not shape or shape[-1] != K or W.dtype is not self._w or W.shape != self._w_shape
+                or not W.is_contiguous() or scale_a.dtype is not torch.float32 or scale_a.shape != lead + (kb,) or scale_w.dtype is not torch.float32
+                or scale_w.shape != self._sw_shape or not scale_w.is_contiguous() or W.get_device() != dev or scale_a.get_device() != dev
+                or scale_w.get_device() != dev):
+            self._refuse(A, W, scale_a, scale_w, bias, output)
+        w_ptr = W.data_ptr()
+        if w_ptr & 15 or (bias is not None) is not self._with_bias:
+            self._refuse(A, W, scale_a, scale_w, bias, output)
+        if bias is None:
+            bias_ptr = None
+        else:
+            if bias.dtype is not self._out or bias.shape != self._bias_shape or not bias.is_contiguous() or bias.get_device() != dev:
+                self._refuse(A, W, scale_a, scale_w, bias, output)
+            bias_ptr = bias.data_ptr()
+        if torch.is_grad_enabled():
+            _refuse_grad("BlockScaledMatmul", A, scale_a, scale_w, bias)
         if output is None:
-            output = torch.empty(lead + (N,), dtype=self._out, device=device)
-        elif output.shape != lead + (N,) or output.dtype != self._out or not output.is_contiguous() or output.device != device:
-            raise ValueError(f"output is a contiguous {tuple(lead) + (N,)} tensor in {self._out} on A's device")
+            output = torch.empty(lead + (N,), dtype=self._out, device=A.device)
+        elif output.shape != lead + (N,) or output.dtype is not self._out or not output.is_contiguous() or output.get_device() != dev:
+            self._refuse(A, W, scale_a, scale_w, bias, output)
+        m = A.numel() // K
         if m == 0:
             return output
-        scale_a, ld = _scale_rows(scale_a, m, kb)
-        need = self.workspace_bytes(m)
-        ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
-        status = self._fn(self._ref, A.data_ptr(), W.data_ptr(), scale_a.data_ptr(), ld, scale_w.data_ptr(), bias.data_ptr() if bias is not None else None,
-                          output.data_ptr(), m, ws.data_ptr() if need else None, need, _lib.current_stream_handle(device))
+        if not A.is_contiguous():
+            A = A.contiguous()
+        a_ptr = A.data_ptr()
+        if a_ptr & 15:
+            A = A.clone()
+            a_ptr = A.data_ptr()
+        if len(lead) != 1 or scale_a.stride() != (1, m):
+            scale_a, ld = _scale_rows(scale_a, m, kb)
+        else:
+            ld = m
+        need = self._need.get(m)
+        if need is None:
+            need = self.workspace_bytes(m)
+        if need:
+            ws = torch.empty(need, dtype=torch.uint8, device=A.device)
+            status = self._fn(self._ref, a_ptr, w_ptr, scale_a.data_ptr(), ld, scale_w.data_ptr(), bias_ptr, output.data_ptr(), m, ws.data_ptr(), need,
+                              _raw_stream(dev))
+        else:
+            status = self._fn(self._ref, a_ptr, w_ptr, scale_a.data_ptr(), ld, scale_w.data_ptr(), bias_ptr, output.data_ptr(), m, None, 0, _raw_stream(dev))
         if status != _lib.OK:
             _lib.check(status)
         return output
+
+    __call__ = forward
 
 
 def quantize_blocks(x: torch.Tensor, dtype: str = "e4m3_float8", *, tile: bool = False, gate: Optional[torch.Tensor] = None,
@@ -254,49 +313,47 @@ def quantize_blocks(x: torch.Tensor, dtype: str = "e4m3_float8", *, tile: bool =
 
     scale = max(max|x|, 2^-40) / L, L the largest value of `dtype` (448, 57344); value = x / scale, the float32 quotient, rounded to
     nearest even.  A block of zeros comes back as zeros, one that holds an infinity or a NaN as NaN with a scale that is not finite."""
-    if dtype not in _FP8:
+    qt = _FP8_TYPE.get(dtype)
+    if qt is None:
         raise ValueError(f"dtype is one of {_FP8}")
-    device = x.device
-    if device.type != "cuda":
+    dev = x.get_device()
+    shape, xt = x.shape, x.dtype
+    if dev < 0:
         raise RuntimeError("quantize_blocks runs on the GPU only")
-    if x.dtype not in (torch.float16, torch.bfloat16, torch.float32) or x.dim() < 1 or x.shape[-1] == 0:
-        raise ValueError(f"x is (..., K) in float16, bfloat16 or float32: got {tuple(x.shape)} in {x.dtype}")
-    if tile and (x.dim() != 2 or gate is not None):
+    if xt not in _FLOATS or not shape or shape[-1] == 0:
+        raise ValueError(f"x is (..., K) in float16, bfloat16 or float32: got {tuple(shape)} in {xt}")
+    if tile and (len(shape) != 2 or gate is not None):
         raise ValueError("tiles are taken of an (N, K) tensor, without a gate")
-    if gate is not None and (gate.shape != x.shape or gate.dtype != x.dtype or gate.device != device):
+    if gate is not None and (gate.shape != shape or gate.dtype is not xt or gate.get_device() != dev):
         raise ValueError("gate has the shape, type and device of x")
-    _refuse_grad("quantize_blocks", x, gate)
-    shape, K = x.shape, x.shape[-1]
-    lead = shape[:-1]
+    if torch.is_grad_enabled():
+        _refuse_grad("quantize_blocks", x, gate)
+    K, lead = shape[-1], shape[:-1]
     m = x.numel() // K
-    kb = _blocks(K)
-    qt = torch_dtype(dtype)
+    kb = -(-K // BLOCK)
     if output is None:
+        device = x.device
         q = torch.empty(shape, dtype=qt, device=device)
         s = torch.empty((_blocks(m), kb), dtype=torch.float32, device=device) if tile else _new_scales(lead, m, kb, device)
+        ld = m
     else:
         q, s = output
-        if q.shape != shape or q.dtype != qt or not q.is_contiguous() or q.device != device:
+        if q.shape != shape or q.dtype is not qt or not q.is_contiguous() or q.get_device() != dev:
             raise ValueError(f"output values are a contiguous {tuple(shape)} tensor in {qt} on x's device")
         want = (_blocks(m), kb) if tile else lead + (kb,)
-        if s.shape != want or s.dtype != torch.float32 or s.device != device or (tile and not s.is_contiguous()):
+        if s.shape != want or s.dtype is not torch.float32 or s.get_device() != dev or (tile and not s.is_contiguous()):
             raise ValueError(f"output scales are a {tuple(want)} tensor in float32 on x's device")
+        ld = m if tile or m == 0 else _scale_ld(s, lead, m, kb)
     if m == 0:
         return q, s
-    a = BlockQuant()
-    if not tile:
-        flat, a.s_ld = _scale_rows(s, m, kb)
-        if flat.data_ptr() != s.data_ptr():
-            raise ValueError("output scales have the rows of a block side by side, as quantize_blocks returns them")
-    a.struct_size = ctypes.sizeof(BlockQuant)
-    a.x_dtype, a.q_dtype, a.tile = _CODE[x.dtype], _CODE[qt], int(tile)
-    a.rows, a.K = m, K
-    x, a.x_ld = _rows(x)
+    x, x_ld = _rows(x)
+    a = BlockQuant(_QUANT_BYTES, _CODE[xt], _CODE[qt], tile, m, K, x_ld)
+    a.s_ld = ld
     a.X, a.Q, a.S = x.data_ptr(), q.data_ptr(), s.data_ptr()
     if gate is not None:
         gate, a.gate_ld = _rows(gate)
         a.gate = gate.data_ptr()
-    status = _library().wqaa_block_quantize(ctypes.byref(a), _lib.current_stream_handle(device))
+    status = _library().wqaa_block_quantize(a, _raw_stream(dev))
     if status != _lib.OK:
         _lib.check(status)
     return q, s
@@ -332,6 +389,13 @@ def _gate_rows(gate: torch.Tensor, x: torch.Tensor) -> Tuple[torch.Tensor, int, 
     return g, ld, share
 
 
+def _check_norm_weight(w: torch.Tensor, name: str, D: int, t: torch.dtype, wt: torch.dtype, dev: int) -> None:
+    d = w.dtype
+    if w.shape != (D,) or d is not wt or (d is not t and d is not torch.float32) or not w.is_contiguous() or w.get_device() != dev:
+        raise ValueError(f"{name} is a contiguous ({D},) tensor in {t} or float32 on x's device (weight and post_weight of one type): "
+                         f"got {tuple(w.shape)} in {d} on {w.device}")
+
+
 def residual_norm(x: torch.Tensor, residual: Optional[torch.Tensor] = None, weight: Optional[torch.Tensor] = None, eps: float = 1e-6, *,
                   post_weight: Optional[torch.Tensor] = None, gate: Optional[torch.Tensor] = None, scale: float = 1.0, residual_scale: float = 1.0,
                   quantize: Optional[str] = None, output: Optional[Sequence[Optional[torch.Tensor]]] = None
@@ -353,81 +417,78 @@ def residual_norm(x: torch.Tensor, residual: Optional[torch.Tensor] = None, weig
     Returns (h, y), h in the residual's type.  Without residual, gate, post_weight and scale, h is x and is returned as it is.  float32
     inside; y is taken of h before h is rounded, and every output is rounded once.  (The reference's norm,
     integration/BitNet/modeling_bitnet.py:89-104, rounds to the activations' type before it multiplies by the weight.)"""
-    device = x.device
-    if device.type != "cuda":
+    dev = x.get_device()
+    if dev < 0:
         raise RuntimeError("residual_norm runs on the GPU only")
-    t = x.dtype
-    if t not in (torch.float16, torch.bfloat16) or x.dim() < 1 or not 1 <= x.shape[-1] <= 32768:
-        raise ValueError(f"x is (..., D) in float16 or bfloat16, D <= 32768: got {tuple(x.shape)} in {t}")
-    shape, D = x.shape, x.shape[-1]
-    st = t
+    t, shape = x.dtype, x.shape
+    if (t is not torch.float16 and t is not torch.bfloat16) or not shape or not 1 <= shape[-1] <= 32768:
+        raise ValueError(f"x is (..., D) in float16 or bfloat16, D <= 32768: got {tuple(shape)} in {t}")
+    D = shape[-1]
+    st = wt = t
     if residual is not None:
         st = residual.dtype
-        if residual.shape != shape or st not in (t, torch.float32):
-            raise ValueError(f"residual has x's shape, in {t} or float32: got {tuple(residual.shape)} in {st}")
-    wt = None
-    for name, w in (("weight", weight), ("post_weight", post_weight)):
-        if w is None:
-            continue
-        if w.shape != (D,) or w.dtype not in (t, torch.float32) or not w.is_contiguous():
-            raise ValueError(f"{name} is a contiguous ({D},) tensor in {t} or float32")
-        if wt is not None and w.dtype != wt:
-            raise ValueError("weight and post_weight have one type")
-        wt = w.dtype
-    if gate is not None and gate.dtype != t:
-        raise ValueError(f"gate is in {t}")
-    if quantize is not None and (quantize not in _FP8 or weight is None):
-        raise ValueError(f"quantize is one of {_FP8}, and goes with a weight")
-    if not float(eps) >= 0.0:
+        if residual.shape != shape or (st is not t and st is not torch.float32) or residual.get_device() != dev:
+            raise ValueError(f"residual has x's shape and device, in {t} or float32: got {tuple(residual.shape)} in {st} on {residual.device}")
+    if weight is not None:
+        wt = weight.dtype
+        _check_norm_weight(weight, "weight", D, t, wt, dev)
+    if post_weight is not None:
+        if weight is None:
+            wt = post_weight.dtype
+        _check_norm_weight(post_weight, "post_weight", D, t, wt, dev)
+    if gate is not None and (gate.dtype is not t or gate.get_device() != dev):
+        raise ValueError(f"gate is in {t}, on x's device")
+    yt = t
+    if quantize is not None:
+        yt = _FP8_TYPE.get(quantize)
+        if yt is None or weight is None:
+            raise ValueError(f"quantize is one of {_FP8}, and goes with a weight")
+    if not eps >= 0.0:
         raise ValueError("the norm's eps must be a non-negative number")
-    _on("residual_norm", device, ("residual", residual), ("weight", weight), ("post_weight", post_weight), ("gate", gate))
-    _refuse_grad("residual_norm", x, residual, weight, post_weight, gate)
-    m = x.numel() // D
-    kb = _blocks(D)
+    if torch.is_grad_enabled():
+        _refuse_grad("residual_norm", x, residual, weight, post_weight, gate)
     passes = residual is None and gate is None and post_weight is None and scale == 1.0     # h is x
     if passes and weight is None:
         raise ValueError("nothing to do: no residual, gate, post_weight or scale, and no weight")
-    out = (None,) * 3 if output is None else (tuple(output) + (None,) * 3)[:3]
-    h, y, s = out
-    if h is None:
-        h = x if passes else torch.empty(shape, dtype=st, device=device)
-        write_h = not passes
-    else:
-        if h.shape != shape or h.dtype != st or not h.is_contiguous() or h.device != device:
+    m = x.numel() // D
+    kb = -(-D // BLOCK)
+    lead = shape[:-1]
+    h = y = s = None
+    ld = m
+    if output is not None:
+        h, y, s = (tuple(output) + (None,) * 3)[:3]
+        if h is not None and (h.shape != shape or h.dtype is not st or not h.is_contiguous() or h.get_device() != dev):
             raise ValueError(f"output h is a contiguous {tuple(shape)} tensor in {st} on x's device")
-        write_h = True
-    yt = t if quantize is None else torch_dtype(quantize)
+        if y is not None and (weight is None or y.shape != shape or y.dtype is not yt or not y.is_contiguous() or y.get_device() != dev):
+            raise ValueError(f"output y goes with a weight and is a contiguous {tuple(shape)} tensor in {yt} on x's device")
+        if s is not None:
+            if quantize is None or s.shape != lead + (kb,) or s.dtype is not torch.float32 or s.get_device() != dev:
+                raise ValueError(f"output scales go with quantize and are a {tuple(lead) + (kb,)} tensor in float32 on x's device")
+            ld = _scale_ld(s, lead, m, kb) if m else m
+    write_h = h is not None or not passes
+    if h is None:
+        h = x if passes else torch.empty(shape, dtype=st, device=x.device)
     if weight is None:
-        if y is not None or s is not None:
-            raise ValueError("an output for y goes with a weight")
+        result = (h, None)
     else:
         if y is None:
-            y = torch.empty(shape, dtype=yt, device=device)
-        elif y.shape != shape or y.dtype != yt or not y.is_contiguous() or y.device != device:
-            raise ValueError(f"output y is a contiguous {tuple(shape)} tensor in {yt} on x's device")
+            y = torch.empty(shape, dtype=yt, device=x.device)
         if quantize is None:
-            if s is not None:
-                raise ValueError("an output for scales goes with quantize")
-        elif s is None:
-            s = _new_scales(shape[:-1], m, kb, device)
-        elif s.shape != shape[:-1] + (kb,) or s.dtype != torch.float32 or s.device != device:
-            raise ValueError(f"output scales are a {tuple(shape[:-1]) + (kb,)} tensor in float32 on x's device")
-    result = (h, None if weight is None else y if quantize is None else (y, s))
+            result = (h, y)
+        else:
+            if s is None:
+                s = _new_scales(lead, m, kb, x.device)
+            result = (h, (y, s))
     if m == 0:
         return result
-    a = ResidualNormArgs()
-    a.struct_size = ctypes.sizeof(ResidualNormArgs)
-    a.x_dtype, a.stream_dtype, a.weight_dtype = _CODE[t], _CODE[st], _CODE[wt or t]
-    a.q_dtype = -1 if quantize is None else _CODE[yt]
-    a.eps, a.scale, a.residual_scale = float(eps), float(scale), float(residual_scale)
-    a.rows, a.D = m, D
-    x, a.x_ld = _rows(x)
+    x, x_ld = _rows(x)
+    a = ResidualNormArgs(_NORM_BYTES, _CODE[t], _CODE[st], _CODE[wt], -1 if quantize is None else _CODE[yt], eps, scale, residual_scale, m, D, x_ld)
     a.x = x.data_ptr()
     if residual is not None:
         residual, a.residual_ld = _rows(residual)
         a.residual = residual.data_ptr()
     if gate is not None:
-        gate, a.gate_ld, a.gate_rows = _gate_rows(gate, result[0])
+        gate, a.gate_ld, a.gate_rows = _gate_rows(gate, h)
         a.gate = gate.data_ptr()
     if post_weight is not None:
         a.post_weight = post_weight.data_ptr()
@@ -436,11 +497,8 @@ def residual_norm(x: torch.Tensor, residual: Optional[torch.Tensor] = None, weig
     if weight is not None:
         a.weight, a.Y = weight.data_ptr(), y.data_ptr()
         if quantize is not None:
-            flat, a.s_ld = _scale_rows(s, m, kb)
-            if flat.data_ptr() != s.data_ptr():
-                raise ValueError("output scales have the rows of a block side by side, as quantize_blocks returns them")
-            a.S = s.data_ptr()
-    status = _library().wqaa_residual_norm(ctypes.byref(a), _lib.current_stream_handle(device))
+            a.S, a.s_ld = s.data_ptr(), ld
+    status = _library().wqaa_residual_norm(a, _raw_stream(dev))
     if status != _lib.OK:
         _lib.check(status)
     return result

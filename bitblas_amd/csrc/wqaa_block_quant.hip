@@ -119,13 +119,17 @@ __device__ __forceinline__ float block_scale(uint32_t amax_bits, int q_dtype) {
 // x / s for 8 values of a block, rounded to 8 bits.  r = 1 / s correctly rounded once per block; x r is within an ulp of the
 // quotient, its remainder x - (x r) s is exact in one fma, and adding remainder * r gives the correctly rounded quotient
 // (P. Markstein, IBM J. Res. Dev. 34, 1990): 3 operations a value instead of a division.  s is infinite or NaN: the remainder is NaN.
-__device__ __forceinline__ u32x2_t quantise8(const float (&v)[8], float s, int q_dtype) {
+// LO: the value is v + lo, lo what v's own rounding lost; it joins the remainder.
+template <bool LO = false>
+__device__ __forceinline__ u32x2_t quantise8(const float (&v)[8], float s, int q_dtype, const float* lo = nullptr) {
   const float r = 1.f / s;
   float q[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     const float t = v[e] * r;
-    q[e] = __builtin_fmaf(__builtin_fmaf(-t, s, v[e]), r, t);
+    float rest = __builtin_fmaf(-t, s, v[e]);
+    if constexpr (LO) rest += lo[e];
+    q[e] = __builtin_fmaf(rest, r, t);
   }
   int w[2] = {0, 0};
 #pragma unroll
@@ -279,17 +283,20 @@ __global__ void __launch_bounds__(1024) wq_residual_norm_kernel(const NormArgs n
     for (int w = 0; w < waves; ++w) t += part[which][w];
     return t;
   };
-  auto times_weight = [&](const void* w, float r) {
+  auto load_weight = [&](const void* w, int v, float (&wt)[8]) {
+    if (a.weight_dtype == WQAA_F32) load8<WQAA_F32, VEC>(w, col[v], n[v], wt);
+    else load8<DT, VEC>(w, col[v], n[v], wt);
+  };
+  if (a.post_weight) {
+    const float r = 1.f / sqrtf(row_mean(0) + a.eps);
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
       float wt[8];
-      if (a.weight_dtype == WQAA_F32) load8<WQAA_F32, VEC>(w, col[v], n[v], wt);
-      else load8<DT, VEC>(w, col[v], n[v], wt);
+      load_weight(a.post_weight, v, wt);
 #pragma unroll
       for (int e = 0; e < 8; ++e) h[v][e] = h[v][e] * r * wt[e];
     }
-  };
-  if (a.post_weight) times_weight(a.post_weight, 1.f / sqrtf(row_mean(0) + a.eps));
+  }
   if (a.gate) {
     const long grow = row / a.gate_rows * a.gate_ld;
 #pragma unroll
@@ -310,14 +317,24 @@ __global__ void __launch_bounds__(1024) wq_residual_norm_kernel(const NormArgs n
     if (a.stream) store8<ST, VEC>(a.stream, row * a.D + col[v], n[v], h[v]);
   }
   if (!a.Y) return;
-  times_weight(a.weight, 1.f / sqrtf(row_mean(1) + a.eps));
+  const float r = 1.f / sqrtf(row_mean(1) + a.eps);
 #pragma unroll
   for (int v = 0; v < NV; ++v) {
+    float y[8], lo[8];
+    load_weight(a.weight, v, y);
+    // h r w in two products; what they round off (lo) matters only next to a border between two 8-bit values, where it decides
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float c = r * y[e];
+      const float p = h[v][e] * c;
+      lo[e] = __builtin_fmaf(h[v][e], c, -p) + h[v][e] * __builtin_fmaf(r, y[e], -c);
+      y[e] = p;
+    }
     if (a.q_dtype < 0) {
-      store8<DT, VEC>(a.Y, row * a.D + col[v], n[v], h[v]);
+      store8<DT, VEC>(a.Y, row * a.D + col[v], n[v], y);
     } else {
-      const float s = block_scale(row_max(abs_max8(h[v])), a.q_dtype);
-      store_q<VEC>(reinterpret_cast<unsigned char*>(a.Y) + row * a.D + col[v], n[v], quantise8(h[v], s, a.q_dtype));
+      const float s = block_scale(row_max(abs_max8(y)), a.q_dtype);
+      store_q<VEC>(reinterpret_cast<unsigned char*>(a.Y) + row * a.D + col[v], n[v], quantise8<true>(y, s, a.q_dtype, lo));
       if ((threadIdx.x & 15) == 0 && n[v] > 0) a.S[col[v] / kBlock * a.s_ld + row] = s;
     }
   }
