@@ -7,7 +7,7 @@ namespace wqaa {
 namespace {
 
 struct Choice {
-  int stream_waves;      // > 0: the streaming member with this many waves
+  int stream;            // > 0: the streaming member, which form of it (stream_form)
   int bm;                // tile members: activation rows of a tile (256: the ping-pong member, whose tiles are 256 weight rows wide)
   int tiles_m, tiles_n, whole, split, split_len;   // workgroups: whole + (tiles_m tiles_n - whole) split
   long tail() const { return (long)tiles_m * tiles_n - whole; }
@@ -17,9 +17,15 @@ struct Choice {
 Choice choose(const wqaa_block_desc& d, int m) {
   Choice c = {};
   const int kb = (d.K + kBlock - 1) / kBlock;
-  if (m <= 16) {
-    c.stream_waves = kb >= 16 ? 8 : 4;
-    c.tiles_m = 1, c.tiles_n = (d.N + 15) / 16, c.whole = c.tiles_n, c.split = 1, c.split_len = kb;
+  // few rows: W streams once.  Weight fragments of a wave (nf): at more than 4 rows the activations' reads weigh as much as W's, and a wave
+  // that takes 4 (2) fragments cuts them to a quarter (half) as long as the workgroups still fill the chip: 16 x 28672 x 8192 47 us with 4, 54
+  // with 2, 57 with 1; 16 x 8192 x 28672 45 us with 2, 57 with 1, 68 with 4; 16 x 4096 x 4096 6.0 us with 1, 7.4 with 2; one row 39.5 us with 1,
+  // 48 with 2 (28672 x 8192).  33 ... 64 rows: 64 x 4096 x 4096 12 us against 20 for tiles and their partial sums; 64 x 8192 x 8192 38 against 27.
+  if (m <= 32 || (m <= 64 && d.N <= 6144)) {
+    const int nf = m <= 4 || m > 32 ? 1 : d.N >= 10240 ? 4 : d.N >= 7168 ? 2 : 1;
+    if (m <= 16) c.stream = nf == 4 ? 4 : nf == 2 ? 3 : kb >= 64 ? 2 : 1;
+    else c.stream = m > 32 ? 8 : nf == 4 ? 7 : nf == 2 ? 6 : 5;
+    c.tiles_m = 1, c.tiles_n = (d.N + 16 * nf - 1) / (16 * nf), c.whole = c.tiles_n, c.split = 1, c.split_len = kb;
     return c;
   }
   {
@@ -67,10 +73,22 @@ void init_pair() {
   tile_attr<BlockTile<WF, AF, 64, 3>>();
   tile_attr<BlockTile<WF, AF, 128, 2>>();
 }
+struct StreamForm {
+  int waves, nf;
+};
+// one row 28672 x 8192: 16 waves, one block ahead 38.8 us, 8 waves, 4 blocks at once 39.5; 4096 x 4096 5.0 and 4.7
+constexpr StreamForm kStream[] = {{0, 0}, {8, 1}, {16, 1}, {16, 2}, {8, 4}, {8, 1}, {8, 2}, {8, 4}, {8, 1}};
 template <int WF, int AF>
 void launch_pair(const Choice& c, const BlockGemmArgs& a, hipStream_t s) {
-  if (c.stream_waves == 8) wq_block_stream_kernel<WF, AF, 8><<<dim3(a.tiles_n), dim3(512), 0, s>>>(a);
-  else if (c.stream_waves == 4) wq_block_stream_kernel<WF, AF, 4><<<dim3(a.tiles_n), dim3(256), 0, s>>>(a);
+  const dim3 g(a.tiles_n), t(kStream[c.stream].waves * 64);
+  if (c.stream == 1) wq_block_stream_kernel<WF, AF, 8, 4, 1, 1, false><<<g, t, 0, s>>>(a);
+  else if (c.stream == 2) wq_block_stream_kernel<WF, AF, 16, 1, 1, 1, true><<<g, t, 0, s>>>(a);
+  else if (c.stream == 3) wq_block_stream_kernel<WF, AF, 16, 1, 2, 1, true><<<g, t, 0, s>>>(a);
+  else if (c.stream == 4) wq_block_stream_kernel<WF, AF, 8, 1, 4, 1, true><<<g, t, 0, s>>>(a);
+  else if (c.stream == 5) wq_block_stream_kernel<WF, AF, 8, 1, 1, 2, true><<<g, t, 0, s>>>(a);
+  else if (c.stream == 6) wq_block_stream_kernel<WF, AF, 8, 1, 2, 2, true><<<g, t, 0, s>>>(a);
+  else if (c.stream == 7) wq_block_stream_kernel<WF, AF, 8, 1, 4, 2, true><<<g, t, 0, s>>>(a);
+  else if (c.stream == 8) wq_block_stream_kernel<WF, AF, 8, 1, 1, 4, true><<<g, t, 0, s>>>(a);
   else if (c.bm == 32) tile_go<BlockTile<WF, AF, 32, 3>>(c, a, s);
   else if (c.bm == 64) tile_go<BlockTile<WF, AF, 64, 3>>(c, a, s);
   else if (c.bm == 128) tile_go<BlockTile<WF, AF, 128, 2>>(c, a, s);
@@ -97,14 +115,14 @@ int block_gemm_plan(const wqaa_block_desc& d, int m, wqaa_plan* plan) {
   const Choice c = choose(d, m);
   memset(plan, 0, sizeof(*plan));
   plan->kernel_family = 2;
-  plan->block_m = c.stream_waves ? 16 : c.bm;
-  plan->block_n = c.stream_waves ? 16 : c.bm == 256 ? 256 : 128;
+  plan->block_m = c.stream ? (m + 15) / 16 * 16 : c.bm;
+  plan->block_n = c.stream ? kStream[c.stream].nf * 16 : c.bm == 256 ? 256 : 128;
   plan->block_k = kBlock;
-  plan->threads = c.stream_waves ? c.stream_waves * 64 : c.bm == 256 ? BlockPP::THREADS : 256;
+  plan->threads = c.stream ? kStream[c.stream].waves * 64 : c.bm == 256 ? BlockPP::THREADS : 256;
   plan->grid = (int)c.grid();
   plan->split_k = c.split;
   snprintf(plan->name, sizeof(plan->name), "block_matmul_m%dn%dk%d_%sx%s_%s%dx%d%s", m, d.N, d.K, short_dtype(d.a_dtype), short_dtype(d.w_dtype),
-           c.stream_waves ? "stream" : c.bm == 256 ? "pp" : "tile", plan->block_m, plan->block_n, c.split > 1 ? "_split" : "");
+           c.stream ? "stream" : c.bm == 256 ? "pp" : "tile", plan->block_m, plan->block_n, c.split > 1 ? "_split" : "");
   return WQAA_OK;
 }
 

@@ -42,72 +42,148 @@ __device__ __forceinline__ void block_store1(void* C, int dt, long i, float v) {
   else reinterpret_cast<uint16_t*>(C)[i] = block_bf16(v);
 }
 
-// ---- m <= 16: the weights stream through registers --------------------------------------------------------------------------------
-// One read of W is all there is to do, so nothing is shared and nothing is staged: a wave takes 16 weight rows and every WAVES-th
-// k-block of them straight into the matrix operand's registers (two 16-byte loads a lane), the activations - one fragment of 16 rows, from
-// L2 - the same way; the waves' partial tiles meet in LDS in a fixed order.  Rows beyond m and n repeat the last one and are not stored.
-template <int WF, int AF, int WAVES>
+// ---- few rows: the weights stream through registers ------------------------------------------------------------------------------
+// One read of W is nearly all there is to do, so nothing is staged: a wave takes NF fragments of 16 weight rows and every WAVES-th
+// k-block of them straight into the matrix operand's registers (two 16-byte loads a lane and fragment), the MF fragments of activation rows -
+// from L2 - the same way; the waves' partial tiles meet in LDS in a fixed order.  Rows beyond m and n repeat the last one and are
+// not stored.  U blocks are asked for at once; PF: the next U before the matrix instructions of these.  NF > 1 divides the reads of the
+// activations, which at 16 rows are as many as those of the weights (choose() in wqaa_block_gemm.hip has the measured rule).
+template <int WF, int AF, int WAVES, int U, int NF, int MF, bool PF>
 __global__ void __launch_bounds__(WAVES * 64) wq_block_stream_kernel(const BlockGemmArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
-  __shared__ float part[WAVES][256];
+  __shared__ __attribute__((aligned(16))) float part[WAVES][NF * 256];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 15, q = lane >> 4;
-  const int n0 = blockIdx.x * 16;
-  const unsigned char* wp = a.W + (long)min(n0 + r, a.N - 1) * a.K + q * 16;
-  const int m = min(r, a.M - 1);
-  const unsigned char* ap = a.A + (long)m * a.K + q * 16;
-  const float* swp = a.sw + (long)(n0 / kBlock) * a.KB;
-  const float* sap = a.sa + m;
-  bf32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  const int full = a.K / kBlock;                 // blocks that are whole
-  constexpr int U = 4;
-  int b = wave;
-  for (; b + (U - 1) * WAVES < full; b += U * WAVES) {
-    bi32x4 w[U][2], x[U][2];
-    float s[U];
+  const int n0 = blockIdx.x * 16 * NF;           // (16 NF divides 128: the rows of a workgroup share a weight tile's scales)
+  const unsigned char* wp[NF];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const long k = (long)(b + u * WAVES) * kBlock;
-      w[u][0] = *reinterpret_cast<const bi32x4*>(wp + k);
-      w[u][1] = *reinterpret_cast<const bi32x4*>(wp + k + 64);
-      x[u][0] = *reinterpret_cast<const bi32x4*>(ap + k);
-      x[u][1] = *reinterpret_cast<const bi32x4*>(ap + k + 64);
-      s[u] = sap[(long)(b + u * WAVES) * a.sa_ld] * swp[b + u * WAVES];
-    }
+  for (int g = 0; g < NF; ++g) wp[g] = a.W + (long)min(n0 + g * 16 + r, a.N - 1) * a.K + q * 16;
+  const unsigned char* ap[MF];
+  const float* sap[MF];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const bf32x4 d = block_mfma<WF, AF>(w[u], x[u]);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) acc[i] = __builtin_fmaf(d[i], s[u], acc[i]);
-    }
+  for (int f = 0; f < MF; ++f) {
+    const int m = min(f * 16 + r, a.M - 1);
+    ap[f] = a.A + (long)m * a.K + q * 16;
+    sap[f] = a.sa + m;
   }
-  for (; b < a.KB; b += WAVES) {
+  const auto* swp = (const __attribute__((address_space(4))) float*)(a.sw + (long)(n0 / kBlock) * a.KB);
+  bf32x4 acc[MF][NF];
+#pragma unroll
+  for (int f = 0; f < MF; ++f)
+#pragma unroll
+    for (int g = 0; g < NF; ++g) acc[f][g] = bf32x4{0.f, 0.f, 0.f, 0.f};
+  struct Batch {
+    bi32x4 w[U][NF][2], x[U][MF][2];
+    float sa[U][MF], sw[U];
+  };
+  auto piece = [](const unsigned char* p) { return *reinterpret_cast<const bi32x4*>(p); };
+  auto fetch = [&](Batch& B, int u, int b) {     // block b, whole
     const long k = (long)b * kBlock;
-    const int left = a.K - b * kBlock - q * 16;  // pieces beyond K are zero in both operands
-    bi32x4 w[2] = {}, x[2] = {};
-    if (left > 0) w[0] = *reinterpret_cast<const bi32x4*>(wp + k), x[0] = *reinterpret_cast<const bi32x4*>(ap + k);
-    if (left > 64) w[1] = *reinterpret_cast<const bi32x4*>(wp + k + 64), x[1] = *reinterpret_cast<const bi32x4*>(ap + k + 64);
-    const float s = sap[(long)b * a.sa_ld] * swp[b];
-    const bf32x4 d = block_mfma<WF, AF>(w, x);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) acc[i] = __builtin_fmaf(d[i], s, acc[i]);
+    for (int g = 0; g < NF; ++g) B.w[u][g][0] = piece(wp[g] + k), B.w[u][g][1] = piece(wp[g] + k + 64);
+#pragma unroll
+    for (int f = 0; f < MF; ++f) {
+      B.x[u][f][0] = piece(ap[f] + k), B.x[u][f][1] = piece(ap[f] + k + 64);
+      B.sa[u][f] = sap[f][(long)b * a.sa_ld];
+    }
+    B.sw[u] = swp[b];
+  };
+  auto multiply = [&](const Batch& B) {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int f = 0; f < MF; ++f) {
+        const float s = B.sa[u][f] * B.sw[u];
+#pragma unroll
+        for (int g = 0; g < NF; ++g) {
+          const bf32x4 d = block_mfma<WF, AF>(B.w[u][g], B.x[u][f]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[f][g][i] = __builtin_fmaf(d[i], s, acc[f][g][i]);
+        }
+      }
+  };
+  const int full = a.K / kBlock;                 // blocks that are whole
+  const int cnt = full > wave ? (full - wave + WAVES - 1) / WAVES : 0;
+  const int nb = cnt / U;
+  auto batch = [&](Batch& B, int i) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) fetch(B, u, wave + (i * U + u) * WAVES);
+  };
+  if constexpr (PF) {
+    Batch even, odd;
+    if (nb > 0) batch(even, 0);
+    int i = 0;
+    for (; i + 2 < nb; i += 2) {
+      batch(odd, i + 1);
+      __builtin_amdgcn_sched_barrier(0);
+      multiply(even);
+      __builtin_amdgcn_sched_barrier(0);
+      batch(even, i + 2);
+      __builtin_amdgcn_sched_barrier(0);
+      multiply(odd);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if (i + 1 < nb) {
+      batch(odd, i + 1);
+      __builtin_amdgcn_sched_barrier(0);
+      multiply(even);
+      multiply(odd);
+    } else if (nb > 0) {
+      multiply(even);
+    }
+  } else {
+    for (int i = 0; i < nb; ++i) {
+      Batch B;
+      batch(B, i);
+      __builtin_amdgcn_sched_barrier(0);
+      multiply(B);
+    }
+  }
+  if (nb * U < cnt) {                            // fewer than U blocks left: the others are zero
+    Batch B = {};
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (nb * U + u < cnt) fetch(B, u, wave + (nb * U + u) * WAVES);
+    multiply(B);
+  }
+  if (full < a.KB && full % WAVES == wave) {     // the last block holds fewer than 128 k: pieces beyond K are zero in both operands
+    const long k = (long)full * kBlock;
+    const int left = a.K - full * kBlock - q * 16;
+    Batch B = {};
+#pragma unroll
+    for (int g = 0; g < NF; ++g) {
+      if (left > 0) B.w[0][g][0] = piece(wp[g] + k);
+      if (left > 64) B.w[0][g][1] = piece(wp[g] + k + 64);
+    }
+#pragma unroll
+    for (int f = 0; f < MF; ++f) {
+      if (left > 0) B.x[0][f][0] = piece(ap[f] + k);
+      if (left > 64) B.x[0][f][1] = piece(ap[f] + k + 64);
+      B.sa[0][f] = sap[f][(long)full * a.sa_ld];
+    }
+    B.sw[0] = swp[full];
+    multiply(B);
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) part[wave][r * 16 + q * 4 + i] = acc[i];
-  __syncthreads();
-  for (int t = threadIdx.x; t < 256; t += WAVES * 64) {
-    const int mm = t >> 4, n = n0 + (t & 15);
-    if (mm >= a.M || n >= a.N) continue;
-    float v = 0.f;
+  for (int f = 0; f < MF; ++f) {                 // one fragment row of the partial tiles at a time
+    if (f) __syncthreads();
 #pragma unroll
-    for (int wv = 0; wv < WAVES; ++wv) v += part[wv][t];
-    if (a.bias) v += block_bias(a.bias, a.out_dtype, n);
-    block_store1(a.C, a.out_dtype, (long)mm * a.N + n, v);
+    for (int g = 0; g < NF; ++g) *reinterpret_cast<bf32x4*>(&part[wave][r * (16 * NF) + g * 16 + q * 4]) = acc[f][g];
+    __syncthreads();
+    for (int t = threadIdx.x; t < 256 * NF; t += WAVES * 64) {
+      const int m = f * 16 + t / (16 * NF), n = n0 + t % (16 * NF);
+      if (m >= a.M || n >= a.N) continue;
+      float v = 0.f;
+#pragma unroll
+      for (int wv = 0; wv < WAVES; ++wv) v += part[wv][t];
+      if (a.bias) v += block_bias(a.bias, a.out_dtype, n);
+      block_store1(a.C, a.out_dtype, (long)m * a.N + n, v);
+    }
   }
 #endif
 }
 
-// ---- m > 16: tiles of BM x 128 through LDS ------------------------------------------------------------------------------------------
+// ---- more rows: tiles of BM x 128 through LDS ------------------------------------------------------------------------------------------
 // Four waves, S stages of one k-block each, every byte by LDS-DMA.  A stage holds BM activation rows and 128 weight rows of 128 bytes,
 // 16-byte piece g of row r at slot g ^ ((r >> 1) & 7) (the lanes of an operand read then hit every bank twice, which is the rate),
 // and per wave the scales of its own activation rows (64 of them; rows beyond M read as zero).  Half a CU's LDS at most: two
