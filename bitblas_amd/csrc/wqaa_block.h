@@ -18,8 +18,7 @@ struct BlockGemmArgs {
   int M, N, K, KB;                           // KB = ceil(K / 128)
   int out_dtype;                             // wqaa_dtype
   int tiles_m, tiles_n;
-  int whole;                                 // tiles with a workgroup of their own; each tile behind them is shared by `split`
-  int split, split_len;                      // k-blocks [z * split_len, min(KB, (z + 1) * split_len)) for slice z
+  int split, split_len;                      // workgroups of a tile: slice z takes k-blocks [z * split_len, min(KB, (z + 1) * split_len))
   int group_m;                               // M-tiles that share an N-tile back to back
 };
 

@@ -9,9 +9,9 @@ namespace {
 struct Choice {
   int stream;            // > 0: the streaming member, which form of it (stream_form)
   int bm;                // tile members: activation rows of a tile (256: the ping-pong member, whose tiles are 256 weight rows wide)
-  int tiles_m, tiles_n, whole, split, split_len;   // workgroups: whole + (tiles_m tiles_n - whole) split
-  long tail() const { return (long)tiles_m * tiles_n - whole; }
-  long grid() const { return whole + tail() * split; }
+  int tiles_m, tiles_n, split, split_len;
+  long tiles() const { return (long)tiles_m * tiles_n; }
+  long grid() const { return tiles() * split; }
 };
 
 Choice choose(const wqaa_block_desc& d, int m) {
@@ -25,31 +25,37 @@ Choice choose(const wqaa_block_desc& d, int m) {
     const int nf = m <= 4 || m > 32 ? 1 : d.N >= 10240 ? 4 : d.N >= 7168 ? 2 : 1;
     if (m <= 16) c.stream = nf == 4 ? 4 : nf == 2 ? 3 : kb >= 64 ? 2 : 1;
     else c.stream = m > 32 ? 8 : nf == 4 ? 7 : nf == 2 ? 6 : 5;
-    c.tiles_m = 1, c.tiles_n = (d.N + 16 * nf - 1) / (16 * nf), c.whole = c.tiles_n, c.split = 1, c.split_len = kb;
+    c.tiles_m = 1, c.tiles_n = (d.N + 16 * nf - 1) / (16 * nf), c.split = 1, c.split_len = kb;
     return c;
   }
-  {
-    const long tiles = (long)((m + 255) / 256) * ((d.N + 255) / 256);
-    if (m > 128 && tiles >= 192) {
-      c.bm = 256;
-      c.tiles_m = (m + 255) / 256, c.tiles_n = (d.N + 255) / 256;
-      c.whole = (int)tiles, c.split = 1, c.split_len = kb;
-      return c;
+  auto tiles_of = [&](int bm, int bn) {
+    c.bm = bm, c.tiles_m = (m + bm - 1) / bm, c.tiles_n = (d.N + bn - 1) / bn;
+    c.split = 1, c.split_len = kb;
+    return (long)c.tiles_m * c.tiles_n;
+  };
+  // many rows: the ping-pong member, where its 256 x 256 tiles (one a CU) leave less than about a third of their last round empty:
+  // 1024 x 11008 x 4096, 172 tiles, 66 us against 69 for 128-row tiles; 4096 x 5120 x 5120, 320 tiles, 131 against 125;
+  // 2048 x 11008 x 4096, 344 tiles, 109 against 113; 2048 x 28672 x 8192, 896 tiles, 435 against 517
+  const long big = tiles_of(256, 256), rounds = (big + 255) / 256;
+  if (m > 128 && big * 20 >= rounds * 256 * 13) return c;
+  // tiles of 64 rows up to two a CU, of 128 rows beyond: 1024 x 4096 x 4096, 512 tiles of 64, 27 us against 32; 700 x 8192 x 4096, 704
+  // of them, 43 against 37
+  const long small = tiles_of(64, kBlock);
+  if (small > 512) {
+    (void)tiles_of(128, kBlock);
+    return c;
+  }
+  // few of them: K in slices that fill the chip once, of at least 4 blocks, at most 8 - the partial tiles cost their way to memory and
+  // back: 128 x 4096 x 4096, 64 tiles, 4 slices 13 us, 2 15 us, 8 over 16 us; 512 x 1024 x 4096, 64 tiles, 4 14.5 us, none 20 us
+  if (small < 160) {
+    long split = 256 / small;
+    if (split > 8) split = 8;
+    if (split > kb / 4) split = kb / 4;
+    if (split > 1) {
+      c.split_len = (int)((kb + split - 1) / split);
+      c.split = (kb + c.split_len - 1) / c.split_len;
     }
   }
-  c.bm = m <= 32 ? 32 : m <= 64 ? 64 : 128;
-  c.tiles_m = (m + c.bm - 1) / c.bm;
-  c.tiles_n = (d.N + kBlock - 1) / kBlock;
-  // whole rounds of the chip (a tile per CU) take tiles with a workgroup of their own; what is left over is cut along K, in slices of
-  // at least 2 blocks, so that it fills the chip once and not a last round of whole tiles
-  const long tiles = (long)c.tiles_m * c.tiles_n;
-  long rest = tiles % 256;
-  long split = rest ? 512 / rest : 1;
-  if (split > kb / 2) split = kb / 2;
-  if (split < 2 || tiles > 4096) split = 1, rest = 0;
-  c.whole = (int)(tiles - rest);
-  c.split_len = (int)((kb + split - 1) / split);
-  c.split = (kb + c.split_len - 1) / c.split_len;
   return c;
 }
 
@@ -69,7 +75,6 @@ template <int WF, int AF>
 void init_pair() {
   pp_attr<WF, AF, false>();
   pp_attr<WF, AF, true>();
-  tile_attr<BlockTile<WF, AF, 32, 3>>();
   tile_attr<BlockTile<WF, AF, 64, 3>>();
   tile_attr<BlockTile<WF, AF, 128, 2>>();
 }
@@ -89,7 +94,6 @@ void launch_pair(const Choice& c, const BlockGemmArgs& a, hipStream_t s) {
   else if (c.stream == 6) wq_block_stream_kernel<WF, AF, 8, 1, 2, 2, true><<<g, t, 0, s>>>(a);
   else if (c.stream == 7) wq_block_stream_kernel<WF, AF, 8, 1, 4, 2, true><<<g, t, 0, s>>>(a);
   else if (c.stream == 8) wq_block_stream_kernel<WF, AF, 8, 1, 1, 4, true><<<g, t, 0, s>>>(a);
-  else if (c.bm == 32) tile_go<BlockTile<WF, AF, 32, 3>>(c, a, s);
   else if (c.bm == 64) tile_go<BlockTile<WF, AF, 64, 3>>(c, a, s);
   else if (c.bm == 128) tile_go<BlockTile<WF, AF, 128, 2>>(c, a, s);
   else if (a.K % kBlock) wq_block_pp_kernel<WF, AF, true><<<dim3(a.tiles_m * a.tiles_n), dim3(BlockPP::THREADS), BlockPP::LDS, s>>>(a);
@@ -107,7 +111,7 @@ void block_init() {
 
 size_t block_gemm_workspace_bytes(const wqaa_block_desc& d, int m) {
   const Choice c = choose(d, m);
-  return c.split > 1 ? (size_t)c.tail() * c.split * c.bm * kBlock * 4 : 0;
+  return c.split > 1 ? (size_t)c.tiles() * c.split * c.bm * kBlock * 4 : 0;
 }
 
 int block_gemm_plan(const wqaa_block_desc& d, int m, wqaa_plan* plan) {
@@ -145,14 +149,14 @@ int block_gemm_launch(const wqaa_block_desc& d, const void* A, const void* W, co
   a.C = C, a.ws = reinterpret_cast<float*>(workspace);
   a.M = m, a.N = d.N, a.K = d.K, a.KB = (d.K + kBlock - 1) / kBlock;
   a.out_dtype = d.out_dtype;
-  a.tiles_m = c.tiles_m, a.tiles_n = c.tiles_n, a.whole = c.whole, a.split = c.split, a.split_len = c.split_len;
+  a.tiles_m = c.tiles_m, a.tiles_n = c.tiles_n, a.split = c.split, a.split_len = c.split_len;
   a.group_m = c.tiles_m < 8 ? c.tiles_m : 8;
   const int wf = d.w_dtype == WQAA_E5M2, af = d.a_dtype == WQAA_E5M2;
   if (wf == 0 && af == 0) launch_pair<0, 0>(c, a, stream);
   else if (wf == 0) launch_pair<0, 1>(c, a, stream);
   else if (af == 0) launch_pair<1, 0>(c, a, stream);
   else launch_pair<1, 1>(c, a, stream);
-  if (c.split > 1) wq_block_reduce_kernel<<<dim3((unsigned)(c.tail() * (c.bm / 8))), dim3(256), 0, stream>>>(a, c.bm);
+  if (c.split > 1) wq_block_reduce_kernel<<<dim3((unsigned)(c.tiles() * (c.bm / 8))), dim3(256), 0, stream>>>(a, c.bm);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) {
     set_error(WQAA_ERR_LAUNCH, "block_matmul: %s", hipGetErrorString(e));

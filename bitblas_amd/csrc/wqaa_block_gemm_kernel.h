@@ -188,12 +188,11 @@ __global__ void __launch_bounds__(WAVES * 64) wq_block_stream_kernel(const Block
 // 16-byte piece g of row r at slot g ^ ((r >> 1) & 7) (the lanes of an operand read then hit every bank twice, which is the rate),
 // and per wave the scales of its own activation rows (64 of them; rows beyond M read as zero).  Half a CU's LDS at most: two
 // workgroups share a CU, and one's copies and operand reads run under the other's matrix instructions.
-// The grid is `whole` workgroups of one tile each, then `split` workgroups for each of the remaining tiles: those that would start
-// another round of the chip take a K slice each and leave float32 partial tiles for the reduce launch behind this one.
+// split > 1: that many workgroups take a K slice of the tile each and leave float32 partial tiles for the reduce launch behind this one.
 template <int WF_, int AF_, int BM_, int S_>
 struct BlockTile {
   static constexpr int WF = WF_, AF = AF_, BM = BM_, BN = 128, S = S_, THREADS = 256;
-  static constexpr int WM = BM >= 64 ? 2 : 1, WN = 4 / WM;               // wave grid
+  static constexpr int WM = 2, WN = 2;                                   // wave grid
   static constexpr int MF = BM / WM / 16, NF = BN / WN / 16;             // fragments of a wave
   static constexpr int A_BYTES = BM * 128, W_BYTES = BN * 128, SC_BYTES = 4 * 256;
   static constexpr int STAGE = A_BYTES + W_BYTES + SC_BYTES;
@@ -238,16 +237,10 @@ __global__ void __launch_bounds__(P::THREADS, 2) wq_block_tile_kernel(const Bloc
   const int r = lane & 15, q = lane >> 4;
   const int wm = wave / P::WN, wn = wave % P::WN;
 
-  int tile_m, tile_n, b_first = 0, b_end = a.KB, piece = -1;
-  if ((int)blockIdx.x < a.whole) {
-    block_tile_of(a, blockIdx.x, a.whole, tile_m, tile_n);
-  } else {
-    piece = blockIdx.x - a.whole;
-    const int t = piece / a.split;
-    b_first = (piece - t * a.split) * a.split_len;
-    b_end = min(a.KB, b_first + a.split_len);
-    block_tile_of(a, a.whole + t, 1, tile_m, tile_n);
-  }
+  int tile_m, tile_n;
+  const int tile = blockIdx.x / a.split, slice = blockIdx.x - tile * a.split;
+  block_tile_of(a, tile, a.tiles_m * a.tiles_n, tile_m, tile_n);
+  const int b_first = slice * a.split_len, b_end = min(a.KB, b_first + a.split_len);
   const int m0 = tile_m * P::BM, n0 = tile_n * P::BN;
 
   // tile-relative buffers: the range ends with the matrix, so rows beyond it read as zero
@@ -272,9 +265,8 @@ __global__ void __launch_bounds__(P::THREADS, 2) wq_block_tile_kernel(const Bloc
 #pragma unroll
     for (int j = 0; j < P::AP; ++j) {
       const int row = wave * (P::BM / 4) + j * 8;
-      const bool odd = P::BM == 32 ? (wave & 1) : (j & 1);
-      const uint32_t v = va + (uint32_t)(j * 8) * (uint32_t)a.K + (odd ? k1 : k0);
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(a_rsrc, (lds_t)(base + row * 128), 16, (odd ? out1 : out0) ? OUT : v, b * kBlock, 0, 0);
+      const uint32_t v = va + (uint32_t)(j * 8) * (uint32_t)a.K + ((j & 1) ? k1 : k0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(a_rsrc, (lds_t)(base + row * 128), 16, ((j & 1) ? out1 : out0) ? OUT : v, b * kBlock, 0, 0);
     }
 #pragma unroll
     for (int j = 0; j < P::WP; ++j) {
@@ -344,8 +336,8 @@ __global__ void __launch_bounds__(P::THREADS, 2) wq_block_tile_kernel(const Bloc
 #pragma unroll
     for (int g = 0; g < P::NF; ++g) {
       const int nl = (wn * P::NF + g) * 16 + q * 4, n = n0 + nl;
-      if (piece >= 0) {                           // a slice: the whole tile, rows and columns beyond the matrix included
-        *reinterpret_cast<bf32x4*>(a.ws + ((long)piece * P::BM + ml) * P::BN + nl) = acc[f][g];
+      if (a.split > 1) {                          // a slice: the whole tile, rows and columns beyond the matrix included
+        *reinterpret_cast<bf32x4*>(a.ws + (((long)tile * a.split + slice) * P::BM + ml) * P::BN + nl) = acc[f][g];
         continue;
       }
       if (m >= a.M || n >= a.N) continue;
@@ -374,7 +366,7 @@ __global__ void __launch_bounds__(256) wq_block_reduce_kernel(const BlockGemmArg
   const int per_tile = bm / 8;
   const int t = blockIdx.x / per_tile, part = blockIdx.x % per_tile;
   int tile_m, tile_n;
-  block_tile_of(a, a.whole + t, 1, tile_m, tile_n);
+  block_tile_of(a, t, a.tiles_m * a.tiles_n, tile_m, tile_n);
   const int ml = part * 8 + (threadIdx.x >> 5), nl = (threadIdx.x & 31) * 4;
   const int m = tile_m * bm + ml, n = tile_n * kBlock + nl;
   if (m >= a.M || n >= a.N) return;
