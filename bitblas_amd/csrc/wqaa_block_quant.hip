@@ -157,7 +157,22 @@ __device__ __forceinline__ void store_q(unsigned char* q, int n, u32x2_t w) {
   }
 }
 
-__device__ __forceinline__ float silu(float g) { return g * __builtin_amdgcn_rcpf(1.f + __expf(-g)); }
+// silu(g) * u = u g / (1 + 2^(-g log2 e)), within about two roundings: the exponent's argument in two parts, the reciprocal with one
+// Newton step, and in `lo` what the two products round off.  (A value next to a border between two 8-bit values is decided by
+// that: with a plain exponential and reciprocal some ten times as many values fell on the other side.)
+__device__ __forceinline__ float gated(float g, float u, float& lo) {
+  constexpr float kL = 1.44269502f, kLLo = 1.92596299e-8f;               // log2 e = kL + kLLo
+  const float t = -g * kL;
+  const float t_lo = __builtin_fmaf(-g, kL, -t) - g * kLLo;
+  const float e2 = __builtin_amdgcn_exp2f(t);
+  const float y = 1.f + __builtin_fmaf(e2 * t_lo, 0.693147182f, e2);
+  const float r0 = __builtin_amdgcn_rcpf(y);
+  const float r = t < 120.f ? __builtin_fmaf(__builtin_fmaf(-y, r0, 1.f), r0, r0) : __builtin_amdgcn_rcpf(1.f + e2);   // (2^t is or nears infinity: 0)
+  const float c = g * r;
+  const float p = c * u;
+  lo = __builtin_fmaf(c, u, -p) + __builtin_fmaf(g, r, -c) * u;
+  return p;
+}
 
 struct QuantArgs {
   const void* x;
@@ -184,6 +199,7 @@ __global__ void __launch_bounds__(256) wq_block_quant_rows_kernel(const QuantArg
     const long row = r0 + i * 4 + (g >> 2);
     load8<DT, VEC>(a.x, row * a.x_ld + col, row < a.rows ? n : 0, x[i]);
   }
+  float lo[4][8];
   if constexpr (GATED) {
     float gt[4][8];
 #pragma unroll
@@ -194,13 +210,13 @@ __global__ void __launch_bounds__(256) wq_block_quant_rows_kernel(const QuantArg
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[i][e] = silu(gt[i][e]) * x[i][e];
+      for (int e = 0; e < 8; ++e) x[i][e] = gated(gt[i][e], x[i][e], lo[i][e]);
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const long row = r0 + i * 4 + (g >> 2);
     const float s = block_scale(row_max(abs_max8(x[i])), a.q_dtype);
-    const u32x2_t w = quantise8(x[i], s, a.q_dtype);
+    const u32x2_t w = quantise8<GATED>(x[i], s, a.q_dtype, lo[i]);
     if (row < a.rows) {
       store_q<VEC>(a.q + row * a.K + col, n, w);
       if (l == 0 && b < a.kb) a.s[(long)b * a.s_ld + row] = s;
