@@ -75,8 +75,10 @@ template <int WF, int AF>
 void init_pair() {
   pp_attr<WF, AF, false>();
   pp_attr<WF, AF, true>();
-  tile_attr<BlockTile<WF, AF, 64, 3>>();
-  tile_attr<BlockTile<WF, AF, 128, 2>>();
+  tile_attr<BlockTile<WF, AF, 64, 3, false>>();
+  tile_attr<BlockTile<WF, AF, 64, 3, true>>();
+  tile_attr<BlockTile<WF, AF, 128, 2, false>>();
+  tile_attr<BlockTile<WF, AF, 128, 2, true>>();
 }
 struct StreamForm {
   int waves, nf;
@@ -85,6 +87,7 @@ struct StreamForm {
 constexpr StreamForm kStream[] = {{0, 0}, {8, 1}, {16, 1}, {16, 2}, {8, 4}, {8, 1}, {8, 2}, {8, 4}, {8, 1}};
 template <int WF, int AF>
 void launch_pair(const Choice& c, const BlockGemmArgs& a, hipStream_t s) {
+  const bool tail = a.K % kBlock != 0;
   const dim3 g(a.tiles_n), t(kStream[c.stream].waves * 64);
   if (c.stream == 1) wq_block_stream_kernel<WF, AF, 8, 4, 1, 1, false><<<g, t, 0, s>>>(a);
   else if (c.stream == 2) wq_block_stream_kernel<WF, AF, 16, 1, 1, 1, true><<<g, t, 0, s>>>(a);
@@ -94,9 +97,11 @@ void launch_pair(const Choice& c, const BlockGemmArgs& a, hipStream_t s) {
   else if (c.stream == 6) wq_block_stream_kernel<WF, AF, 8, 1, 2, 2, true><<<g, t, 0, s>>>(a);
   else if (c.stream == 7) wq_block_stream_kernel<WF, AF, 8, 1, 4, 2, true><<<g, t, 0, s>>>(a);
   else if (c.stream == 8) wq_block_stream_kernel<WF, AF, 8, 1, 1, 4, true><<<g, t, 0, s>>>(a);
-  else if (c.bm == 64) tile_go<BlockTile<WF, AF, 64, 3>>(c, a, s);
-  else if (c.bm == 128) tile_go<BlockTile<WF, AF, 128, 2>>(c, a, s);
-  else if (a.K % kBlock) wq_block_pp_kernel<WF, AF, true><<<dim3(a.tiles_m * a.tiles_n), dim3(BlockPP::THREADS), BlockPP::LDS, s>>>(a);
+  else if (c.bm == 64 && tail) tile_go<BlockTile<WF, AF, 64, 3, true>>(c, a, s);
+  else if (c.bm == 64) tile_go<BlockTile<WF, AF, 64, 3, false>>(c, a, s);
+  else if (c.bm == 128 && tail) tile_go<BlockTile<WF, AF, 128, 2, true>>(c, a, s);
+  else if (c.bm == 128) tile_go<BlockTile<WF, AF, 128, 2, false>>(c, a, s);
+  else if (tail) wq_block_pp_kernel<WF, AF, true><<<dim3(a.tiles_m * a.tiles_n), dim3(BlockPP::THREADS), BlockPP::LDS, s>>>(a);
   else wq_block_pp_kernel<WF, AF, false><<<dim3(a.tiles_m * a.tiles_n), dim3(BlockPP::THREADS), BlockPP::LDS, s>>>(a);
 }
 

@@ -189,8 +189,10 @@ __global__ void __launch_bounds__(WAVES * 64) wq_block_stream_kernel(const Block
 // and per wave the scales of its own activation rows (64 of them; rows beyond M read as zero).  Half a CU's LDS at most: two
 // workgroups share a CU, and one's copies and operand reads run under the other's matrix instructions.
 // split > 1: that many workgroups take a K slice of the tile each and leave float32 partial tiles for the reduce launch behind this one.
-template <int WF_, int AF_, int BM_, int S_>
+// TAIL: K is no multiple of 128 (pieces of the last block beyond K are fetched from outside the buffer, which reads as zero)
+template <int WF_, int AF_, int BM_, int S_, bool TAIL_>
 struct BlockTile {
+  static constexpr bool TAIL = TAIL_;
   static constexpr int WF = WF_, AF = AF_, BM = BM_, BN = 128, S = S_, THREADS = 256;
   static constexpr int WM = 2, WN = 2;                                   // wave grid
   static constexpr int MF = BM / WM / 16, NF = BN / WN / 16;             // fragments of a wave
@@ -259,7 +261,7 @@ __global__ void __launch_bounds__(P::THREADS, 2) wq_block_tile_kernel(const Bloc
   auto stage = [&](int t, int slot) {
     const int b = min(b_first + t, b_end - 1);                           // (beyond the slice: the last block again, never used)
     unsigned char* base = smem + slot * P::STAGE;
-    const bool cut = b == last;
+    const bool cut = P::TAIL && b == last;
     const bool out0 = cut && g0 * 16 >= tail, out1 = cut && g1 * 16 >= tail;
     const uint32_t k0 = g0 * 16, k1 = g1 * 16;
 #pragma unroll
@@ -296,7 +298,6 @@ __global__ void __launch_bounds__(P::THREADS, 2) wq_block_tile_kernel(const Bloc
     const float sw = swp[t];
     block_wait_vm<(P::S - 2) * P::PIECES>();      // this wave's pieces of block t have landed (one kind of load in flight: in order)
     WQ_BLOCK_BARRIER();                           // everyone's have, and everyone is done with block t - 1, whose slot is filled next
-    stage(t + P::S - 1, fill);
     const unsigned char* base = smem + slot * P::STAGE;
     bi32x4 w[P::NF][2], x[P::MF][2];
     float s[P::MF];
@@ -311,8 +312,13 @@ __global__ void __launch_bounds__(P::THREADS, 2) wq_block_tile_kernel(const Bloc
       const unsigned char* p = base + (wm * P::MF + f) * 2048;
       x[f][0] = *reinterpret_cast<const bi32x4*>(p + rd0);
       x[f][1] = *reinterpret_cast<const bi32x4*>(p + rd1);
-      s[f] = reinterpret_cast<const float*>(base + P::A_BYTES + P::W_BYTES + wave * 256)[f * 16 + r] * sw;
+      s[f] = reinterpret_cast<const float*>(base + P::A_BYTES + P::W_BYTES + wave * 256)[f * 16 + r];
     }
+    __builtin_amdgcn_sched_barrier(0);
+    stage(t + P::S - 1, fill);                    // behind the operand reads: its address work runs in their shadow
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int f = 0; f < P::MF; ++f) s[f] *= sw;
     bf32x4 d[3];
 #pragma unroll
     for (int i = 0; i < P::MF * P::NF + 2; ++i) {  // result i's fmas two matrix instructions behind it
