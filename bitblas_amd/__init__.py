@@ -23,7 +23,7 @@ from .module import Linear  # noqa: F401
 from .group import GatedMLP, LinearGroup, gate_up_plan, group_plan, matmul_gate_up, matmul_group  # noqa: F401  (MI355X extension: one launch for q/k/v, gate/up)
 from .chain import ChainStep, DecoderTail, chain_plan, matmul_chain  # noqa: F401  (a chain of dependent operators described once, run as its launches)
 from .block_scaled import (  # noqa: F401  (8-bit operands with a scale per block of 128: product, quantiser, the norms around a block)
-    BlockScaledMatmul, BlockScaledMatmulConfig, quantize_blocks, residual_norm,
+    BlockScaledDecoderTail, BlockScaledGatedMLP, BlockScaledLinear, BlockScaledMatmul, BlockScaledMatmulConfig, quantize_blocks, residual_norm,
 )
 from .cache import (  # noqa: F401
     OperatorCache, get_database_path, global_operator_cache, load_global_ops_cache,

@@ -509,3 +509,112 @@ def residual_norm(x: torch.Tensor, residual: Optional[torch.Tensor] = None, weig
     if status != _lib.OK:
         _lib.check(status)
     return result
+
+
+class BlockScaledLinear(torch.nn.Module):
+    """A linear layer on 8-bit operands with a scale per block of 128: `BlockScaledLinear.from_linear(layer)`, or the buffers of a
+    checkpoint that was quantised that way (`weight` (out, in) in `W_dtype`, `weight_scale` (ceil(out / 128), ceil(in / 128)) float32).
+
+    forward(x): x (..., in) in float16, bfloat16 or float32 is quantised per row and block first; (values, scales), as
+    `quantize_blocks` and `residual_norm(quantize=)` return them, is multiplied as it is."""
+
+    def __init__(self, in_features: int, out_features: int, bias: bool = False, A_dtype: str = "e4m3_float8", W_dtype: str = "e4m3_float8",
+                 out_dtype: str = "float16"):
+        super().__init__()
+        self.in_features, self.out_features = in_features, out_features
+        self.bitblas_matmul = BlockScaledMatmul(BlockScaledMatmulConfig(N=out_features, K=in_features, A_dtype=A_dtype, W_dtype=W_dtype,
+                                                                        out_dtype=out_dtype, with_bias=bias))
+        self.A_dtype, self.W_dtype, self.out_dtype = A_dtype, W_dtype, out_dtype
+        self.register_buffer("weight", torch.zeros((out_features, in_features), dtype=torch_dtype(W_dtype)))
+        self.register_buffer("weight_scale", torch.ones((_blocks(out_features), _blocks(in_features)), dtype=torch.float32))
+        if bias:
+            self.register_buffer("bias", torch.zeros(out_features, dtype=torch_dtype(out_dtype)))
+        else:
+            self.bias = None
+
+    def load_float_weight(self, weight: torch.Tensor, bias: Optional[torch.Tensor] = None) -> None:
+        """Quantise a float weight into this layer's buffers, on the GPU the layer lives on."""
+        if self.weight.device.type != "cuda":
+            raise RuntimeError("load_float_weight quantises on the GPU: move the layer there first")
+        if weight.shape != (self.out_features, self.in_features):
+            raise ValueError(f"weight is ({self.out_features}, {self.in_features}): got {tuple(weight.shape)}")
+        if (bias is not None) != (self.bias is not None):
+            raise ValueError("the bias goes with a layer that has one, and only with it")
+        w = weight.detach().to(self.weight.device)
+        if w.dtype not in _FLOATS:
+            w = w.float()
+        quantize_blocks(w, self.W_dtype, tile=True, output=(self.weight, self.weight_scale))
+        if bias is not None:
+            self.bias.copy_(bias.detach())
+
+    @classmethod
+    def from_linear(cls, linear: torch.nn.Linear, A_dtype: str = "e4m3_float8", W_dtype: str = "e4m3_float8", out_dtype: Optional[str] = None):
+        """a float `nn.Linear` on the GPU -> this layer; out_dtype: the linear's type where it is a 16-bit one, else float16"""
+        if out_dtype is None:
+            out_dtype = "bfloat16" if linear.weight.dtype is torch.bfloat16 else "float16"
+        layer = cls(linear.in_features, linear.out_features, linear.bias is not None, A_dtype, W_dtype, out_dtype).to(linear.weight.device)
+        layer.load_float_weight(linear.weight, linear.bias)
+        return layer
+
+    def forward(self, x, output: Optional[torch.Tensor] = None) -> torch.Tensor:
+        q, s = x if isinstance(x, tuple) else quantize_blocks(x, self.A_dtype)
+        return self.bitblas_matmul(q, self.weight, s, self.weight_scale, self.bias, output)
+
+
+class BlockScaledGatedMLP(torch.nn.Module):
+    """`down(silu(gate(x)) * up(x))` (+ residual) over block-scaled layers, gate and up as ONE product: three launches, or four with a float
+    x, at any row count (`GatedMLP` is the same block over low-bit weights; integration/BitNet/modeling_bitnet.py:209-244).
+
+    gate_up   `BlockScaledLinear(hidden, 2 * inner)`, gate's rows first; down `BlockScaledLinear(inner, hidden)`"""
+
+    def __init__(self, gate_up: BlockScaledLinear, down: BlockScaledLinear):
+        super().__init__()
+        if gate_up.out_features != 2 * down.in_features:
+            raise ValueError(f"gate_up gives {gate_up.out_features} features, down takes {down.in_features}: gate and up are one half each")
+        self.gate_up, self.down = gate_up, down
+
+    @classmethod
+    def from_linears(cls, gate: torch.nn.Linear, up: torch.nn.Linear, down: torch.nn.Linear, **kw):
+        if gate.weight.shape != up.weight.shape or (gate.bias is None) != (up.bias is None):
+            raise ValueError("gate and up have one shape, and both a bias or none")
+        both = torch.nn.Linear(gate.in_features, 2 * gate.out_features, bias=gate.bias is not None, device=gate.weight.device, dtype=gate.weight.dtype)
+        with torch.no_grad():
+            both.weight.copy_(torch.cat([gate.weight, up.weight]))
+            if gate.bias is not None:
+                both.bias.copy_(torch.cat([gate.bias, up.bias]))
+        return cls(BlockScaledLinear.from_linear(both, **kw), BlockScaledLinear.from_linear(down, **kw))
+
+    def forward(self, x, residual: Optional[torch.Tensor] = None, norm=None) -> torch.Tensor:
+        """norm = (weight, eps): x is the hidden state in front of the MLP's norm.  residual: added to the result, as residual_norm does"""
+        if norm is not None:
+            x = residual_norm(x, None, norm[0], norm[1], quantize=self.gate_up.A_dtype)[1]
+        both = self.gate_up(x)
+        inner = self.down.in_features
+        out = self.down(quantize_blocks(both[..., inner:], self.down.A_dtype, gate=both[..., :inner]))
+        return out if residual is None else residual_norm(out, residual)[0]
+
+
+class BlockScaledDecoderTail(torch.nn.Module):
+    """The half of a decoder layer behind its attention, over block-scaled layers (`DecoderTail` is the same over low-bit weights):
+
+        h   = x + post_attention(o_proj(attn))
+        out = h + post_mlp(mlp(norm(h)))
+
+    with the norm in front of the next block too where the caller has its weight: forward(...) -> (out, next_norm(out) or None), the latter
+    quantised and ready for the next layer's projections.  post_attention / post_mlp: weights of norms behind the two blocks, or None."""
+
+    def __init__(self, o_proj: BlockScaledLinear, mlp: BlockScaledGatedMLP, norm_weight: torch.Tensor, eps: float = 1e-6,
+                 post_attention: Optional[torch.Tensor] = None, post_mlp: Optional[torch.Tensor] = None):
+        super().__init__()
+        self.o_proj, self.mlp = o_proj, mlp
+        self.norm_weight, self.post_attention, self.post_mlp = norm_weight, post_attention, post_mlp
+        self.eps = float(eps)
+
+    def forward(self, attn, x: torch.Tensor, next_norm: Optional[torch.Tensor] = None):
+        h, y = residual_norm(self.o_proj(attn), x, self.norm_weight, self.eps, post_weight=self.post_attention, quantize=self.mlp.gate_up.A_dtype)
+        return residual_norm(self.mlp(y), h, next_norm, self.eps, post_weight=self.post_mlp,
+                             quantize=None if next_norm is None else self.mlp.gate_up.A_dtype)
+
+
+__all__ = ["BLOCK", "BlockScaledDecoderTail", "BlockScaledGatedMLP", "BlockScaledLinear", "BlockScaledMatmul", "BlockScaledMatmulConfig",
+           "quantize_blocks", "residual_norm"]

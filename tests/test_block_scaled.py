@@ -112,6 +112,23 @@ def test_host_tensors_are_refused():
             call()
 
 
+def test_layers_without_a_device():
+    """buffers, their state dict, and what a layer refuses"""
+    lin = bitblas.BlockScaledLinear(272, 200, bias=True, out_dtype="bfloat16")
+    assert lin.weight.shape == (200, 272) and lin.weight.dtype == torch.float8_e4m3fn
+    assert lin.weight_scale.shape == (2, 3) and lin.bias.dtype == torch.bfloat16
+    assert set(lin.state_dict()) == {"weight", "weight_scale", "bias"}
+    other = bitblas.BlockScaledLinear(272, 200, bias=True, out_dtype="bfloat16")
+    other.load_state_dict(lin.state_dict())
+    with pytest.raises(RuntimeError, match="GPU"):
+        lin.load_float_weight(torch.zeros(200, 272), torch.zeros(200))
+    with pytest.raises(ValueError):
+        bitblas.BlockScaledLinear(270, 200)
+    with pytest.raises(ValueError):
+        bitblas.BlockScaledGatedMLP(bitblas.BlockScaledLinear(256, 256), bitblas.BlockScaledLinear(256, 256))
+    bitblas.BlockScaledGatedMLP(bitblas.BlockScaledLinear(256, 512), bitblas.BlockScaledLinear(256, 256))
+
+
 def test_row_layouts():
     t = torch.arange(4 * 6 * 10).view(4, 6, 10)
     for view, ld in ((t, 10), (t[:, :, 2:7], 10), (t[1:3, :, :4], 10), (t.view(24, 10)[::2], 20), (t[0], 10), (t[:, 2], 60)):

@@ -500,6 +500,75 @@ def test_a_layer_of_them(rows):
     assert off < 2 * 2 * 2.0 ** -4 / 3 ** 0.5, off.item()
 
 
+def float_tail(seed, D=512, inner=768, dtype=torch.bfloat16):
+    torch.manual_seed(seed)
+    mk = lambda i, o, b=False: torch.nn.Linear(i, o, bias=b, device="cuda", dtype=dtype)  # noqa: E731
+    return mk(D, D, True), mk(D, inner), mk(D, inner), mk(inner, D)
+
+
+@pytest.mark.parametrize("rows", [(1,), (2, 17), (300,)])
+@pytest.mark.parametrize("posts", [False, True])
+def test_decoder_tail(rows, posts):
+    """the modules run the operators they are made of, bit for bit, and stay near the float layers: three quantised products of relative
+    error 2^-4 sqrt(2 / 3) (both operands rounded, uniformly) add up in the branches; twice their root sum of squares is allowed"""
+    D, inner = 512, 768
+    o, gate, up, down = float_tail(1)
+    with torch.no_grad():
+        mlp = bitblas.BlockScaledGatedMLP.from_linears(gate, up, down)
+        o8 = bitblas.BlockScaledLinear.from_linear(o)
+        g = gen(len(rows))
+        w, w2, p1, p2 = ((1 + 0.1 * torch.randn(D, generator=g)).bfloat16().cuda() for _ in range(4))
+        tail = bitblas.BlockScaledDecoderTail(o8, mlp, w, 1e-5, p1 if posts else None, p2 if posts else None)
+        attn, x = (torch.randn(*rows, D, generator=g).bfloat16().cuda() for _ in range(2))
+        out, (q, s) = tail(attn, x, next_norm=w2)
+        # by hand
+        y = o8.bitblas_matmul(*(lambda a: (a[0], o8.weight, a[1], o8.weight_scale))(bitblas.quantize_blocks(attn)), o8.bias)
+        h, y = bitblas.residual_norm(y, x, w, 1e-5, post_weight=p1 if posts else None, quantize="e4m3_float8")
+        both = mlp.gate_up.bitblas_matmul(y[0], mlp.gate_up.weight, y[1], mlp.gate_up.weight_scale)
+        a = bitblas.quantize_blocks(both[..., inner:], gate=both[..., :inner])
+        d = mlp.down.bitblas_matmul(a[0], mlp.down.weight, a[1], mlp.down.weight_scale)
+        want, y2 = bitblas.residual_norm(d, h, w2, 1e-5, post_weight=p2 if posts else None, quantize="e4m3_float8")
+        assert torch.equal(out, want) and torch.equal(q.float(), y2[0].float()) and torch.equal(s, y2[1])
+        plain, none = tail(attn, x)
+        assert none is None and torch.equal(plain, out)
+        # the MLP alone, its norm and its residual
+        full = mlp(h, residual=h, norm=(w, 1e-5))
+        y3 = bitblas.residual_norm(h, None, w, 1e-5, quantize="e4m3_float8")[1]
+        assert torch.equal(full, bitblas.residual_norm(mlp(y3), h)[0])
+        # the float layers in 64 bits
+        rms = lambda t, wt: t / torch.sqrt(t.square().mean(-1, keepdim=True) + 1e-5) * wt.double()  # noqa: E731
+        W = lambda l: l.weight.double().t()  # noqa: E731
+        b1 = attn.double() @ W(o) + o.bias.double()
+        h64 = x.double() + (rms(b1, p1) if posts else b1)
+        n64 = rms(h64, w)
+        act = torch.nn.functional.silu(n64 @ W(gate)) * (n64 @ W(up))
+        b2 = act @ W(down)
+        b2 = rms(b2, p2) if posts else b2
+        allowed = 2 * 3 ** 0.5 * 2.0 ** -4 * (2 / 3) ** 0.5 * (h64 - x.double()).norm().hypot(b2.norm())
+        assert (out.double() - (h64 + b2)).norm() <= allowed
+
+
+def test_linear_layer():
+    torch.manual_seed(3)
+    lin = torch.nn.Linear(400, 300, device="cuda", dtype=torch.float16)
+    layer = bitblas.BlockScaledLinear.from_linear(lin)
+    assert layer.out_dtype == "float16"
+    x = torch.randn(3, 7, 400, device="cuda").half()
+    wq, ws = plain_quantise(lin.weight, "e4m3_float8", tile=True)
+    assert torch.equal(layer.weight.cpu().float(), wq.float()) and torch.equal(layer.weight_scale.cpu(), ws)
+    C = layer(x)
+    q, s = plain_quantise(x, "e4m3_float8")
+    assert C.shape == (3, 7, 300)
+    check_product(C.view(21, 300), q.view(21, 400), wq, s.reshape(21, 4), ws, lin.bias.detach())
+    assert torch.equal(layer(bitblas.quantize_blocks(x)), C)
+    out = torch.empty_like(C)
+    assert layer(x, output=out) is out and torch.equal(out, C)
+    with pytest.raises(ValueError):
+        layer.load_float_weight(torch.zeros(300, 300, device="cuda"), lin.bias)
+    with pytest.raises(ValueError):
+        layer.load_float_weight(lin.weight)
+
+
 @pytest.mark.parametrize("rows", [1, 40, 300])
 def test_captured_and_replayed(rows):
     """a captured layer replayed on new inputs, with eager work between the replays, and a second graph beside it: the eager bits"""
