@@ -7,8 +7,9 @@ namespace wqaa {
 namespace {
 
 struct Choice {
-  int stream;            // > 0: the streaming member, which form of it (stream_form)
+  int stream;            // > 0: the streaming member, which form of it (kStream, launch_pair)
   int bm;                // tile members: activation rows of a tile (256: the ping-pong member, whose tiles are 256 weight rows wide)
+  int groups;            // tile member: groups of four waves in a workgroup (BlockTile::G)
   int tiles_m, tiles_n, split, split_len;
   long tiles() const { return (long)tiles_m * tiles_n; }
   long grid() const { return tiles() * split; }
@@ -38,17 +39,23 @@ Choice choose(const wqaa_block_desc& d, int m) {
   // 2048 x 11008 x 4096, 344 tiles, 109 against 113; 2048 x 28672 x 8192, 896 tiles, 435 against 517
   const long big = tiles_of(256, 256), rounds = (big + 255) / 256;
   if (m > 128 && big * 20 >= rounds * 256 * 13) return c;
-  // tiles of 64 rows up to two a CU, of 128 rows beyond: 1024 x 4096 x 4096, 512 tiles of 64, 27 us against 32; 700 x 8192 x 4096, 704
-  // of them, 43 against 37
-  const long small = tiles_of(64, kBlock);
-  if (small > 512) {
-    (void)tiles_of(128, kBlock);
+  // tiles of 128 rows where they are a tile per CU or nearly, or more than two of 64 rows per CU: 512 x 8192 x 8192, 256 of them, 43 us
+  // against 50 for 512 of 64 rows; 128 x 28672 x 8192, 224 of them, 65 against 70; 700 x 8192 x 4096, 704 of 64 rows, 36 against 41
+  const long t128 = tiles_of(128, kBlock);
+  const bool one_each = t128 >= 192 && t128 <= 256;
+  const long t64 = (long)((m + 63) / 64) * c.tiles_n;
+  if (m > 64 && (one_each || t64 > 512)) {
+    c.groups = one_each ? 2 : 1;
     return c;
   }
-  // few of them: K in slices that fill the chip once, of at least 4 blocks, at most 8 - the partial tiles cost their way to memory and
-  // back: 128 x 4096 x 4096, 64 tiles, 4 slices 13 us, 2 15 us, 8 over 16 us; 512 x 1024 x 4096, 64 tiles, 4 14.5 us, none 20 us
-  if (small < 160) {
-    long split = 256 / small;
+  (void)tiles_of(64, kBlock);
+  // 64 rows: up to a tile per CU two groups of waves on it (512 x 4096 x 4096, 256 tiles, 17.6 us against 19.8; 256 x 8192 x 8192 29 against 32).
+  // Fewer tiles than that: K in slices that fill the chip once, of at least 4 blocks, at most 8 - the partial tiles cost their way to memory
+  // and back: 128 x 4096 x 4096, 64 tiles, 4 slices 13.8 us, 2 slices 14.4, 8 over 16; 128 x 8192 x 8192, 128 tiles, 2 slices of two groups
+  // 19.7 us, 4 slices of one 21.2; 512 x 1024 x 4096, 64 tiles, 4 slices 13.8 us, none 20
+  c.groups = t64 >= 128 && t64 <= 256 ? 2 : 1;
+  if (t64 < 160) {
+    long split = c.groups == 2 ? 2 : 256 / t64;
     if (split > 8) split = 8;
     if (split > kb / 4) split = kb / 4;
     if (split > 1) {
@@ -75,10 +82,14 @@ template <int WF, int AF>
 void init_pair() {
   pp_attr<WF, AF, false>();
   pp_attr<WF, AF, true>();
-  tile_attr<BlockTile<WF, AF, 64, 3, false>>();
-  tile_attr<BlockTile<WF, AF, 64, 3, true>>();
-  tile_attr<BlockTile<WF, AF, 128, 2, false>>();
-  tile_attr<BlockTile<WF, AF, 128, 2, true>>();
+  tile_attr<BlockTile<WF, AF, 64, 3, 1, false>>();
+  tile_attr<BlockTile<WF, AF, 64, 3, 1, true>>();
+  tile_attr<BlockTile<WF, AF, 64, 3, 2, false>>();
+  tile_attr<BlockTile<WF, AF, 64, 3, 2, true>>();
+  tile_attr<BlockTile<WF, AF, 128, 2, 1, false>>();
+  tile_attr<BlockTile<WF, AF, 128, 2, 1, true>>();
+  tile_attr<BlockTile<WF, AF, 128, 2, 2, false>>();
+  tile_attr<BlockTile<WF, AF, 128, 2, 2, true>>();
 }
 struct StreamForm {
   int waves, nf;
@@ -97,10 +108,10 @@ void launch_pair(const Choice& c, const BlockGemmArgs& a, hipStream_t s) {
   else if (c.stream == 6) wq_block_stream_kernel<WF, AF, 8, 1, 2, 2, true><<<g, t, 0, s>>>(a);
   else if (c.stream == 7) wq_block_stream_kernel<WF, AF, 8, 1, 4, 2, true><<<g, t, 0, s>>>(a);
   else if (c.stream == 8) wq_block_stream_kernel<WF, AF, 8, 1, 1, 4, true><<<g, t, 0, s>>>(a);
-  else if (c.bm == 64 && tail) tile_go<BlockTile<WF, AF, 64, 3, true>>(c, a, s);
-  else if (c.bm == 64) tile_go<BlockTile<WF, AF, 64, 3, false>>(c, a, s);
-  else if (c.bm == 128 && tail) tile_go<BlockTile<WF, AF, 128, 2, true>>(c, a, s);
-  else if (c.bm == 128) tile_go<BlockTile<WF, AF, 128, 2, false>>(c, a, s);
+  else if (c.bm == 64 && c.groups == 2) tail ? tile_go<BlockTile<WF, AF, 64, 3, 2, true>>(c, a, s) : tile_go<BlockTile<WF, AF, 64, 3, 2, false>>(c, a, s);
+  else if (c.bm == 64) tail ? tile_go<BlockTile<WF, AF, 64, 3, 1, true>>(c, a, s) : tile_go<BlockTile<WF, AF, 64, 3, 1, false>>(c, a, s);
+  else if (c.bm == 128 && c.groups == 2) tail ? tile_go<BlockTile<WF, AF, 128, 2, 2, true>>(c, a, s) : tile_go<BlockTile<WF, AF, 128, 2, 2, false>>(c, a, s);
+  else if (c.bm == 128) tail ? tile_go<BlockTile<WF, AF, 128, 2, 1, true>>(c, a, s) : tile_go<BlockTile<WF, AF, 128, 2, 1, false>>(c, a, s);
   else if (tail) wq_block_pp_kernel<WF, AF, true><<<dim3(a.tiles_m * a.tiles_n), dim3(BlockPP::THREADS), BlockPP::LDS, s>>>(a);
   else wq_block_pp_kernel<WF, AF, false><<<dim3(a.tiles_m * a.tiles_n), dim3(BlockPP::THREADS), BlockPP::LDS, s>>>(a);
 }
@@ -127,7 +138,7 @@ int block_gemm_plan(const wqaa_block_desc& d, int m, wqaa_plan* plan) {
   plan->block_m = c.stream ? (m + 15) / 16 * 16 : c.bm;
   plan->block_n = c.stream ? kStream[c.stream].nf * 16 : c.bm == 256 ? 256 : 128;
   plan->block_k = kBlock;
-  plan->threads = c.stream ? kStream[c.stream].waves * 64 : c.bm == 256 ? BlockPP::THREADS : 256;
+  plan->threads = c.stream ? kStream[c.stream].waves * 64 : c.bm == 256 ? BlockPP::THREADS : c.groups * 256;
   plan->grid = (int)c.grid();
   plan->split_k = c.split;
   snprintf(plan->name, sizeof(plan->name), "block_matmul_m%dn%dk%d_%sx%s_%s%dx%d%s", m, d.N, d.K, short_dtype(d.a_dtype), short_dtype(d.w_dtype),

@@ -186,22 +186,28 @@ __global__ void __launch_bounds__(WAVES * 64) wq_block_stream_kernel(const Block
 // ---- more rows: tiles of BM x 128 through LDS ------------------------------------------------------------------------------------------
 // Four waves, S stages of one k-block each, every byte by LDS-DMA.  A stage holds BM activation rows and 128 weight rows of 128 bytes,
 // 16-byte piece g of row r at slot g ^ ((r >> 1) & 7) (the lanes of an operand read then hit every bank twice, which is the rate),
-// and per wave the scales of its own activation rows (64 of them; rows beyond M read as zero).  Half a CU's LDS at most: two
-// workgroups share a CU, and one's copies and operand reads run under the other's matrix instructions.
+// and per wave the scales of its own activation rows (64 of them; rows beyond M read as zero).
+// A wave alone on its SIMD spends as long on issuing copies and operand reads as in the matrix unit (neither deeper rings nor operands
+// read a block ahead changed that), so a SIMD gets two:
+//   G = 1  half a CU's LDS at most, and two workgroups share a CU: for grids that give every CU two tiles or more;
+//   G = 2  two such groups of four waves in ONE workgroup, each with its half of the k-blocks and its own ring, one barrier apart: while
+//          one reads operands and issues copies (load phase), the other multiplies.  Their sums meet in LDS at the end.  For grids
+//          of up to a tile per CU.
 // split > 1: that many workgroups take a K slice of the tile each and leave float32 partial tiles for the reduce launch behind this one.
 // TAIL: K is no multiple of 128 (pieces of the last block beyond K are fetched from outside the buffer, which reads as zero)
-template <int WF_, int AF_, int BM_, int S_, bool TAIL_>
+template <int WF_, int AF_, int BM_, int S_, int G_, bool TAIL_>
 struct BlockTile {
   static constexpr bool TAIL = TAIL_;
-  static constexpr int WF = WF_, AF = AF_, BM = BM_, BN = 128, S = S_, THREADS = 256;
+  static constexpr int WF = WF_, AF = AF_, BM = BM_, BN = 128, S = S_, G = G_, THREADS = 256 * G_;
   static constexpr int WM = 2, WN = 2;                                   // wave grid
   static constexpr int MF = BM / WM / 16, NF = BN / WN / 16;             // fragments of a wave
   static constexpr int A_BYTES = BM * 128, W_BYTES = BN * 128, SC_BYTES = 4 * 256;
   static constexpr int STAGE = A_BYTES + W_BYTES + SC_BYTES;
   static constexpr int AP = BM / 32, WP = BN / 32;                       // DMA pieces (8 rows) of a wave per stage
   static constexpr int PIECES = AP + WP + 1;
-  static constexpr int LDS = S * STAGE;
-  static_assert(LDS <= 80 * 1024 && MF * 16 <= 64, "two workgroups a CU; one DMA piece holds a wave's row scales");
+  static constexpr int LDS = G * S * STAGE;
+  static_assert(LDS <= (G == 1 ? 80 : 160) * 1024 && MF * 16 <= 64, "two groups a CU; one DMA piece holds a wave's row scales");
+  static_assert(G == 1 || BM * BN * 4 <= LDS, "the groups' sums meet in LDS");
 };
 
 template <int N>
@@ -231,18 +237,23 @@ __device__ __forceinline__ void block_tile_of(const BlockGemmArgs& a, int blk, i
 }
 
 template <class P>
-__global__ void __launch_bounds__(P::THREADS, 2) wq_block_tile_kernel(const BlockGemmArgs a) {
+__global__ void __launch_bounds__(P::THREADS, 2 / P::G) wq_block_tile_kernel(const BlockGemmArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
   typedef __attribute__((address_space(3))) void* lds_t;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, wave8 = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int grp = wave8 >> 2, wave = wave8 & 3;
   const int r = lane & 15, q = lane >> 4;
   const int wm = wave / P::WN, wn = wave % P::WN;
 
   int tile_m, tile_n;
   const int tile = blockIdx.x / a.split, slice = blockIdx.x - tile * a.split;
   block_tile_of(a, tile, a.tiles_m * a.tiles_n, tile_m, tile_n);
-  const int b_first = slice * a.split_len, b_end = min(a.KB, b_first + a.split_len);
+  const int s_first = slice * a.split_len, s_end = min(a.KB, s_first + a.split_len);
+  // this group's k-blocks: b_first ... b_first + mine - 1; both groups take nt steps
+  const int nt = (s_end - s_first + P::G - 1) / P::G;
+  const int b_first = s_first + grp * nt, mine = min(nt, s_end - b_first);
+  unsigned char* const ring = smem + grp * (P::S * P::STAGE);
   const int m0 = tile_m * P::BM, n0 = tile_n * P::BN;
 
   // tile-relative buffers: the range ends with the matrix, so rows beyond it read as zero
@@ -259,8 +270,8 @@ __global__ void __launch_bounds__(P::THREADS, 2) wq_block_tile_kernel(const Bloc
   const int tail = a.K - last * kBlock;                                  // k in the last block
 
   auto stage = [&](int t, int slot) {
-    const int b = min(b_first + t, b_end - 1);                           // (beyond the slice: the last block again, never used)
-    unsigned char* base = smem + slot * P::STAGE;
+    const int b = min(b_first + t, s_end - 1);                           // (beyond the slice: its last block again, never used)
+    unsigned char* base = ring + slot * P::STAGE;
     const bool cut = P::TAIL && b == last;
     const bool out0 = cut && g0 * 16 >= tail, out1 = cut && g1 * 16 >= tail;
     const uint32_t k0 = g0 * 16, k1 = g1 * 16;
@@ -288,19 +299,12 @@ __global__ void __launch_bounds__(P::THREADS, 2) wq_block_tile_kernel(const Bloc
     for (int g = 0; g < P::NF; ++g) acc[f][g] = bf32x4{0.f, 0.f, 0.f, 0.f};
   const int swl = (r >> 1) & 7;
   const int rd0 = r * 128 + ((q ^ swl) * 16), rd1 = r * 128 + (((4 + q) ^ swl) * 16);
-  const auto* swp = (const __attribute__((address_space(4))) float*)(a.sw + (long)tile_n * a.KB + b_first);
+  const auto* swp = (const __attribute__((address_space(4))) float*)(a.sw + (long)tile_n * a.KB);
 
-  const int nt = b_end - b_first;
-#pragma unroll
-  for (int t = 0; t < P::S - 1; ++t) stage(t, t);
-  int slot = 0, fill = P::S - 1;
-  for (int t = 0; t < nt; ++t) {
-    const float sw = swp[t];
-    block_wait_vm<(P::S - 2) * P::PIECES>();      // this wave's pieces of block t have landed (one kind of load in flight: in order)
-    WQ_BLOCK_BARRIER();                           // everyone's have, and everyone is done with block t - 1, whose slot is filled next
-    const unsigned char* base = smem + slot * P::STAGE;
-    bi32x4 w[P::NF][2], x[P::MF][2];
-    float s[P::MF];
+  bi32x4 w[P::NF][2], x[P::MF][2];
+  float s[P::MF];
+  auto read = [&](int slot) {
+    const unsigned char* base = ring + slot * P::STAGE;
 #pragma unroll
     for (int g = 0; g < P::NF; ++g) {
       const unsigned char* p = base + P::A_BYTES + (wn * P::NF + g) * 2048;
@@ -314,9 +318,8 @@ __global__ void __launch_bounds__(P::THREADS, 2) wq_block_tile_kernel(const Bloc
       x[f][1] = *reinterpret_cast<const bi32x4*>(p + rd1);
       s[f] = reinterpret_cast<const float*>(base + P::A_BYTES + P::W_BYTES + wave * 256)[f * 16 + r];
     }
-    __builtin_amdgcn_sched_barrier(0);
-    stage(t + P::S - 1, fill);                    // behind the operand reads: its address work runs in their shadow
-    __builtin_amdgcn_sched_barrier(0);
+  };
+  auto multiply = [&](float sw) {
 #pragma unroll
     for (int f = 0; f < P::MF; ++f) s[f] *= sw;
     bf32x4 d[3];
@@ -330,11 +333,63 @@ __global__ void __launch_bounds__(P::THREADS, 2) wq_block_tile_kernel(const Bloc
         for (int e = 0; e < 4; ++e) acc[j / P::NF][j % P::NF][e] = __builtin_fmaf(d[j % 3][e], s[j / P::NF], acc[j / P::NF][j % P::NF][e]);
       }
     }
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // (every operand read has long been used: nothing to wait for)
-    slot = slot + 1 == P::S ? 0 : slot + 1;
-    fill = fill + 1 == P::S ? 0 : fill + 1;
+  };
+
+#pragma unroll
+  for (int t = 0; t < P::S - 1; ++t) stage(t, t);
+  int slot = 0, fill = P::S - 1;
+  if constexpr (P::G == 1) {
+    for (int t = 0; t < nt; ++t) {
+      const float sw = swp[b_first + t];
+      block_wait_vm<(P::S - 2) * P::PIECES>();    // this wave's pieces of block t have landed (one kind of load in flight: in order)
+      WQ_BLOCK_BARRIER();                         // everyone's have, and everyone is done with block t - 1, whose slot is filled next
+      read(slot);
+      __builtin_amdgcn_sched_barrier(0);
+      stage(t + P::S - 1, fill);                  // behind the operand reads: its address work runs in their shadow
+      __builtin_amdgcn_sched_barrier(0);
+      multiply(sw);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // (every operand read has long been used: nothing to wait for)
+      slot = slot + 1 == P::S ? 0 : slot + 1;
+      fill = fill + 1 == P::S ? 0 : fill + 1;
+    }
+    block_wait_vm<0>();                           // no DMA into LDS outlives the workgroup
+  } else {
+    block_wait_vm<(P::S - 2) * P::PIECES>();      // block 0
+    WQ_BLOCK_BARRIER();
+    if (grp == 1) WQ_BLOCK_BARRIER();
+    for (int t = 0; t < nt; ++t) {
+      // load phase: block t has landed (the wait and the barrier behind the multiply phase before); the slot that is filled held
+      // block t - 1, which the whole group had read before the barrier of that load phase
+      const float sw = swp[min(b_first + t, s_end - 1)];
+      read(slot);
+      __builtin_amdgcn_sched_barrier(0);
+      stage(t + P::S - 1, fill);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      WQ_BLOCK_BARRIER();
+      if (t < mine) multiply(sw);
+      block_wait_vm<(P::S - 2) * P::PIECES>();    // block t + 1
+      WQ_BLOCK_BARRIER();
+      slot = slot + 1 == P::S ? 0 : slot + 1;
+      fill = fill + 1 == P::S ? 0 : fill + 1;
+    }
+    if (grp == 0) WQ_BLOCK_BARRIER();
+    block_wait_vm<0>();                           // no copy may land in what follows
+    WQ_BLOCK_BARRIER();
+    // the second group's sums through LDS, each lane's own fragments (1 KiB a wave and fragment)
+    unsigned char* const mine_at = smem + wave * (P::MF * P::NF * 1024) + lane * 16;
+    if (grp == 1) {
+#pragma unroll
+      for (int f = 0; f < P::MF; ++f)
+#pragma unroll
+        for (int g = 0; g < P::NF; ++g) *reinterpret_cast<bf32x4*>(mine_at + (f * P::NF + g) * 1024) = acc[f][g];
+    }
+    __syncthreads();
+    if (grp == 1) return;
+#pragma unroll
+    for (int f = 0; f < P::MF; ++f)
+#pragma unroll
+      for (int g = 0; g < P::NF; ++g) acc[f][g] += *reinterpret_cast<const bf32x4*>(mine_at + (f * P::NF + g) * 1024);
   }
-  block_wait_vm<0>();                             // no DMA into LDS outlives the workgroup
 
 #pragma unroll
   for (int f = 0; f < P::MF; ++f) {
