@@ -18,17 +18,26 @@ struct Choice {
 Choice choose(const wqaa_block_desc& d, int m) {
   Choice c = {};
   const int kb = (d.K + kBlock - 1) / kBlock;
-  // few rows: W streams once.  Weight fragments of a wave (nf): at more than 4 rows the activations' reads weigh as much as W's, and a wave
-  // that takes 4 (2) fragments cuts them to a quarter (half) as long as the workgroups still fill the chip: 16 x 28672 x 8192 47 us with 4, 54
-  // with 2, 57 with 1; 16 x 8192 x 28672 45 us with 2, 57 with 1, 68 with 4; 16 x 4096 x 4096 6.0 us with 1, 7.4 with 2; one row 39.5 us with 1,
-  // 48 with 2 (28672 x 8192).  33 ... 64 rows: 64 x 4096 x 4096 12 us against 20 for tiles and their partial sums; 64 x 8192 x 8192 38 against 27.
-  if (m <= 32 || (m <= 64 && d.N <= 6144)) {
-    const int nf = m <= 4 || m > 32 ? 1 : d.N >= 10240 ? 4 : d.N >= 7168 ? 2 : 1;
-    if (m <= 16) c.stream = nf == 4 ? 4 : nf == 2 ? 3 : kb >= 64 ? 2 : 1;
-    else c.stream = m > 32 ? 8 : nf == 4 ? 7 : nf == 2 ? 6 : 5;
-    c.tiles_m = 1, c.tiles_n = (d.N + 16 * nf - 1) / (16 * nf), c.split = 1, c.split_len = kb;
+  auto stream = [&](int form, int rows, int nf) {
+    c.stream = form;
+    c.tiles_m = (m + rows - 1) / rows, c.tiles_n = (d.N + 16 * nf - 1) / (16 * nf), c.split = 1, c.split_len = kb;
     return c;
-  }
+  };
+  // few rows: W streams once.  Weight fragments of a wave: at more than 4 rows the activations' reads weigh as much as W's, and a wave that
+  // takes 4 (2) fragments cuts them to a quarter (half) as long as the workgroups still fill the chip: 16 x 28672 x 8192 47 us with 4, 54
+  // with 2, 57 with 1; 16 x 8192 x 28672 45 us with 2, 57 with 1, 68 with 4; 16 x 4096 x 4096 6.0 us with 1, 7.4 with 2; one row 39.5 us with 1,
+  // 48 with 2 (28672 x 8192).  One fragment: 16 waves a block ahead where each has blocks to run through (one row, 28672 x 8192: 38.8 us
+  // against 39.5 for 8 waves with 4 blocks at once; 4096 x 4096 5.0 against 4.7).
+  if (m <= 16) return m > 4 && d.N >= 10240 ? stream(4, 16, 4) : m > 4 && d.N >= 7168 ? stream(3, 16, 2) : kb >= 64 ? stream(2, 16, 1) : stream(1, 16, 1);
+  // 32 rows a workgroup, more of them along y: small products are through before tiles and their partial sums would be.  One fragment
+  // while that is about a workgroup per CU (77 x 1001 x 1040 3.2 us against 3.8 with two and 8.4 for tiles; 128 x 1024 x 4096 7.7, 9.7 and
+  // 11.1), else two while they take a round of the chip, or two on short K (64 x 4096 x 4096 10.0 us against 13.7 for tiles, 64 x 6144 x 4096
+  // 17.2 against 13.4; 256 x 2048 x 2048 10.0 against 12.0).  Up to 32 rows there is nothing W could be shared with: 24 x 6144 x 4096 9.5 us
+  // with two, 12.0 with one; 32 x 11008 x 4096 14.6 us with four, 17.2 with two.
+  const long chunks = (m + 31) / 32, one = chunks * ((d.N + 15) / 16), two = chunks * ((d.N + 31) / 32), rounds2 = (two + 255) / 256;
+  if (one <= 288 && (m <= 32 || kb <= 48)) return stream(5, 32, 1);
+  if (m <= 32 && d.N >= 10240) return stream(7, 32, 4);
+  if (m <= 32 || (rounds2 <= 2 && rounds2 * kb <= 32)) return stream(6, 32, 2);
   auto tiles_of = [&](int bm, int bn) {
     c.bm = bm, c.tiles_m = (m + bm - 1) / bm, c.tiles_n = (d.N + bn - 1) / bn;
     c.split = 1, c.split_len = kb;
@@ -94,12 +103,11 @@ void init_pair() {
 struct StreamForm {
   int waves, nf;
 };
-// one row 28672 x 8192: 16 waves, one block ahead 38.8 us, 8 waves, 4 blocks at once 39.5; 4096 x 4096 5.0 and 4.7
-constexpr StreamForm kStream[] = {{0, 0}, {8, 1}, {16, 1}, {16, 2}, {8, 4}, {8, 1}, {8, 2}, {8, 4}, {8, 1}};
+constexpr StreamForm kStream[] = {{0, 0}, {8, 1}, {16, 1}, {16, 2}, {8, 4}, {8, 1}, {8, 2}, {8, 4}};
 template <int WF, int AF>
 void launch_pair(const Choice& c, const BlockGemmArgs& a, hipStream_t s) {
   const bool tail = a.K % kBlock != 0;
-  const dim3 g(a.tiles_n), t(kStream[c.stream].waves * 64);
+  const dim3 g(a.tiles_n, a.tiles_m), t(kStream[c.stream].waves * 64);
   if (c.stream == 1) wq_block_stream_kernel<WF, AF, 8, 4, 1, 1, false><<<g, t, 0, s>>>(a);
   else if (c.stream == 2) wq_block_stream_kernel<WF, AF, 16, 1, 1, 1, true><<<g, t, 0, s>>>(a);
   else if (c.stream == 3) wq_block_stream_kernel<WF, AF, 16, 1, 2, 1, true><<<g, t, 0, s>>>(a);
@@ -107,7 +115,6 @@ void launch_pair(const Choice& c, const BlockGemmArgs& a, hipStream_t s) {
   else if (c.stream == 5) wq_block_stream_kernel<WF, AF, 8, 1, 1, 2, true><<<g, t, 0, s>>>(a);
   else if (c.stream == 6) wq_block_stream_kernel<WF, AF, 8, 1, 2, 2, true><<<g, t, 0, s>>>(a);
   else if (c.stream == 7) wq_block_stream_kernel<WF, AF, 8, 1, 4, 2, true><<<g, t, 0, s>>>(a);
-  else if (c.stream == 8) wq_block_stream_kernel<WF, AF, 8, 1, 1, 4, true><<<g, t, 0, s>>>(a);
   else if (c.bm == 64 && c.groups == 2) tail ? tile_go<BlockTile<WF, AF, 64, 3, 2, true>>(c, a, s) : tile_go<BlockTile<WF, AF, 64, 3, 2, false>>(c, a, s);
   else if (c.bm == 64) tail ? tile_go<BlockTile<WF, AF, 64, 3, 1, true>>(c, a, s) : tile_go<BlockTile<WF, AF, 64, 3, 1, false>>(c, a, s);
   else if (c.bm == 128 && c.groups == 2) tail ? tile_go<BlockTile<WF, AF, 128, 2, 2, true>>(c, a, s) : tile_go<BlockTile<WF, AF, 128, 2, 2, false>>(c, a, s);
@@ -135,7 +142,7 @@ int block_gemm_plan(const wqaa_block_desc& d, int m, wqaa_plan* plan) {
   const Choice c = choose(d, m);
   memset(plan, 0, sizeof(*plan));
   plan->kernel_family = 2;
-  plan->block_m = c.stream ? (m + 15) / 16 * 16 : c.bm;
+  plan->block_m = c.stream ? (c.stream <= 4 ? 16 : 32) : c.bm;
   plan->block_n = c.stream ? kStream[c.stream].nf * 16 : c.bm == 256 ? 256 : 128;
   plan->block_k = kBlock;
   plan->threads = c.stream ? kStream[c.stream].waves * 64 : c.bm == 256 ? BlockPP::THREADS : c.groups * 256;

@@ -46,7 +46,7 @@ __device__ __forceinline__ void block_store1(void* C, int dt, long i, float v) {
 // One read of W is nearly all there is to do, so nothing is staged: a wave takes NF fragments of 16 weight rows and every WAVES-th
 // k-block of them straight into the matrix operand's registers (two 16-byte loads a lane and fragment), the MF fragments of activation rows -
 // from L2 - the same way; the waves' partial tiles meet in LDS in a fixed order.  Rows beyond m and n repeat the last one and are
-// not stored.  U blocks are asked for at once; PF: the next U before the matrix instructions of these.  NF > 1 divides the reads of the
+// not stored.  Workgroups along y take 16 MF rows each.  U blocks are asked for at once; PF: the next U before the matrix instructions of these.  NF > 1 divides the reads of the
 // activations, which at 16 rows are as many as those of the weights (choose() in wqaa_block_gemm.hip has the measured rule).
 template <int WF, int AF, int WAVES, int U, int NF, int MF, bool PF>
 __global__ void __launch_bounds__(WAVES * 64) wq_block_stream_kernel(const BlockGemmArgs a) {
@@ -54,6 +54,7 @@ __global__ void __launch_bounds__(WAVES * 64) wq_block_stream_kernel(const Block
   __shared__ __attribute__((aligned(16))) float part[WAVES][NF * 256];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 15, q = lane >> 4;
+  const int m0 = blockIdx.y * 16 * MF, rows = min(16 * MF, a.M - m0);
   const int n0 = blockIdx.x * 16 * NF;           // (16 NF divides 128: the rows of a workgroup share a weight tile's scales)
   const unsigned char* wp[NF];
 #pragma unroll
@@ -62,7 +63,7 @@ __global__ void __launch_bounds__(WAVES * 64) wq_block_stream_kernel(const Block
   const float* sap[MF];
 #pragma unroll
   for (int f = 0; f < MF; ++f) {
-    const int m = min(f * 16 + r, a.M - 1);
+    const int m = m0 + min(f * 16 + r, rows - 1);
     ap[f] = a.A + (long)m * a.K + q * 16;
     sap[f] = a.sa + m;
   }
@@ -172,12 +173,12 @@ __global__ void __launch_bounds__(WAVES * 64) wq_block_stream_kernel(const Block
     __syncthreads();
     for (int t = threadIdx.x; t < 256 * NF; t += WAVES * 64) {
       const int m = f * 16 + t / (16 * NF), n = n0 + t % (16 * NF);
-      if (m >= a.M || n >= a.N) continue;
+      if (m >= rows || n >= a.N) continue;
       float v = 0.f;
 #pragma unroll
       for (int wv = 0; wv < WAVES; ++wv) v += part[wv][t];
       if (a.bias) v += block_bias(a.bias, a.out_dtype, n);
-      block_store1(a.C, a.out_dtype, (long)m * a.N + n, v);
+      block_store1(a.C, a.out_dtype, (long)(m0 + m) * a.N + n, v);
     }
   }
 #endif

@@ -11,8 +11,10 @@
 //     earlier - and A(t + 2) into A(t - 1)'s slot from load segment 0 of block t on.  A wave issues 8 pieces per block in one order, so
 //     "block t + 1 has landed" is vmcnt(8) at the end of segment 1: at most block t + 2's pieces are then in flight, and every other
 //     load of the wave is older than they are or makes the wait stricter;
-//   * row scales: a lane loads the scales of rows lane and 64 + lane of its wave's 128 (two loads a block, a block ahead), and two kinds of
-//     lane swaps hand each fragment's 16 to all four quarter-waves; the weight tile's scale is a scalar.
+//   * row scales: which 16 of a wave's 128 rows a fragment takes is free, and fragment f takes rows 8 r + f: lane r then needs the scales
+//     of 8 neighbouring rows, two 16-byte loads a block (a block ahead) and no exchange between lanes (with rows in order, two 4-byte
+//     loads and lane swaps, 4096 x 28672 x 8192 took 790 us instead of 768); the weight tile's scale is a scalar.  In LDS a fragment's rows
+//     lie together, so the copies permute them: LDS row 16 f + r of a 128-row half holds row 8 r + f.
 #pragma once
 #include "wqaa_block_gemm_kernel.h"
 
@@ -23,18 +25,6 @@ struct BlockPP {
   static constexpr int SLOT = 256 * 128, W_OFF = 3 * SLOT, LDS = 5 * SLOT;
   static_assert(LDS == 160 * 1024 && LDS >= BM * BN * 2, "the rings fill LDS; the epilogue stages the tile there");
 };
-
-// v: lane (r, q) holds row q * 16 + r  ->  out[j]: every lane (r, .) holds row j * 16 + r
-__device__ __forceinline__ void block_spread4(float v, float* out) {
-  const uint32_t u = __builtin_bit_cast(uint32_t, v);
-  const auto h = __builtin_amdgcn_permlane32_swap(u, u, false, false);          // rows 0, 1 twice | rows 2, 3 twice
-  const auto a = __builtin_amdgcn_permlane16_swap(h[0], h[0], false, false);
-  const auto b = __builtin_amdgcn_permlane16_swap(h[1], h[1], false, false);
-  out[0] = __builtin_bit_cast(float, (uint32_t)a[0]);
-  out[1] = __builtin_bit_cast(float, (uint32_t)a[1]);
-  out[2] = __builtin_bit_cast(float, (uint32_t)b[0]);
-  out[3] = __builtin_bit_cast(float, (uint32_t)b[1]);
-}
 
 // TAIL: K is no multiple of 128 (pieces of the last block beyond K are fetched from outside the buffer, which reads as zero)
 template <int WF, int AF, bool TAIL>
@@ -57,26 +47,26 @@ __global__ void __launch_bounds__(BlockPP::THREADS) wq_block_pp_kernel(const Blo
   const auto w_rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(a.W + (long)n0 * a.K), 0, (int)w_bytes, 0x00020000);
   constexpr uint32_t OUT = 0xC0000000u;
   const int g0 = (lane & 7) ^ ((lane >> 4) & 7);
-  const uint32_t rowk = (uint32_t)(wave * 32 + (lane >> 3)) * (uint32_t)a.K;
-  const uint32_t v0 = rowk + g0 * 16, v1 = rowk + (g0 ^ 4) * 16;        // even / odd pieces
+  // first row of the wave's pieces: W's rows in order, A's as LDS rows 32 wave + 8 j + lane / 8 hold them (j & 1: 64 rows on, j / 2: one)
+  const uint32_t w_row = wave * 32 + (lane >> 3), a_row = grp * 128 + (lane >> 3) * 8 + nq * 2;
   const int tail = a.K - (nt - 1) * kBlock;
   const bool cut0 = TAIL && g0 * 16 >= tail, cut1 = TAIL && (g0 ^ 4) * 16 >= tail;
 
-  auto piece = [&](const auto& rsrc, unsigned char* dst, int tt, int j) {
+  auto piece = [&](const auto& rsrc, uint32_t row, unsigned char* dst, int tt, int j) {
     const int tc = min(tt, nt - 1);                                       // (beyond the last block: it again, never used)
-    uint32_t v = ((j & 1) ? v1 : v0) + (uint32_t)(j * 8) * (uint32_t)a.K;
+    uint32_t v = row * (uint32_t)a.K + ((j & 1) ? g0 ^ 4 : g0) * 16;
     if constexpr (TAIL) v = (tc == nt - 1 && ((j & 1) ? cut1 : cut0)) ? OUT : v;
     __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_t)(dst + (wave * 32 + j * 8) * 128), 16, v, tc * kBlock, 0, 0);
   };
-  auto dma_a = [&](int tt, int slot, int j) { piece(a_rsrc, smem + slot * P::SLOT, tt, j); };
-  auto dma_w = [&](int tt, int slot, int j) { piece(w_rsrc, smem + P::W_OFF + slot * P::SLOT, tt, j); };
+  auto dma_a = [&](int tt, int slot, int j) { piece(a_rsrc, a_row + (j & 1) * 64 + (j >> 1), smem + slot * P::SLOT, tt, j); };
+  auto dma_w = [&](int tt, int slot, int j) { piece(w_rsrc, w_row + j * 8, smem + P::W_OFF + slot * P::SLOT, tt, j); };
 
-  const uint32_t srow = (uint32_t)(m0 + grp * 128 + lane) * 4u;
-  float raw[2];
+  const uint32_t srow = (uint32_t)(m0 + grp * 128 + r * 8) * 4u;
+  bf32x4 raw[2];
   auto fetch_scales = [&](int tt) {                                       // rows beyond M are outside the buffer: zero
     const auto rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(a.sa + (long)min(tt, nt - 1) * a.sa_ld), 0, a.M * 4, 0x00020000);
-    raw[0] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rs, srow, 0, 0));
-    raw[1] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rs, srow + 256u, 0, 0));
+    raw[0] = __builtin_bit_cast(bf32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, srow, 0, 0));
+    raw[1] = __builtin_bit_cast(bf32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, srow + 16u, 0, 0));
   };
   const int nb = min((n0 + nq * 64) / kBlock, (a.N - 1) / kBlock);
   const auto* swp = (const __attribute__((address_space(4))) float*)(a.sw + (long)nb * nt);
@@ -103,7 +93,11 @@ __global__ void __launch_bounds__(BlockPP::THREADS) wq_block_pp_kernel(const Blo
   block_wait_vm<8>();
   WQ_BLOCK_BARRIER();
   if (grp == 1) WQ_BLOCK_BARRIER();
-  block_spread4(raw[0] * sw, s);
+  auto scale4 = [&](bf32x4 v, float* to) {
+#pragma unroll
+    for (int f = 0; f < 4; ++f) to[f] = v[f] * sw;
+  };
+  scale4(raw[0], s);
 
   bf32x4 d[3] = {};
   auto scaled = [&](auto PH, int j) {                               // result j of segment PH onto its sums
@@ -134,7 +128,8 @@ __global__ void __launch_bounds__(BlockPP::THREADS) wq_block_pp_kernel(const Blo
       af[f][1] = *reinterpret_cast<const bi32x4*>(as + f * 2048 + rd1);
     }
     const int dslot = slot + 2 >= 3 ? slot - 1 : slot + 2;
-    const float hi = raw[1] * sw;                                         // (segment 0: this block's rows 64 ... 127; segment 1: not used)
+    float hi[4];                                                          // (segment 0: this block's second half; segment 1: not used)
+    scale4(raw[1], hi);
     if constexpr (p == 0) {
       fetch_scales(t + 1);
       sw = swp[min(t + 1, nt - 1)];
@@ -150,8 +145,12 @@ __global__ void __launch_bounds__(BlockPP::THREADS) wq_block_pp_kernel(const Blo
     // are through - the second half's in segment 0, the next block's first half's in segment 1
     __builtin_amdgcn_sched_barrier(0);
     finish(std::integral_constant<int, 1 - p>{});                        // (block 0, segment 0: the results are zero)
-    if constexpr (p == 0) block_spread4(hi, s + 4);
-    else block_spread4(raw[0] * sw, s);
+    if constexpr (p == 0) {
+#pragma unroll
+      for (int f = 0; f < 4; ++f) s[4 + f] = hi[f];
+    } else {
+      scale4(raw[0], s);
+    }
     __builtin_amdgcn_sched_barrier(0);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     if constexpr (p == 1) block_wait_vm<8>();
@@ -180,7 +179,8 @@ __global__ void __launch_bounds__(BlockPP::THREADS) wq_block_pp_kernel(const Blo
   block_wait_vm<0>();                                                     // no copy may land in what the epilogue stages
   WQ_BLOCK_BARRIER();
 
-  // the tile leaves through LDS, whole rows per store: row m at 512 m, its 8-byte unit u (four n) where lanes spread over the banks
+  // the tile leaves through LDS, whole rows per store: row m at 512 m, its 8-byte unit u (four n) at u ^ 4 (m / 8 mod 16) - the 64
+  // lanes of a write, 16 rows 8 apart, then meet every bank twice, and 16-byte pieces stay whole
   const bool f16 = a.out_dtype == WQAA_F16;
 #pragma unroll
   for (int g = 0; g < 4; ++g) {
@@ -192,16 +192,14 @@ __global__ void __launch_bounds__(BlockPP::THREADS) wq_block_pp_kernel(const Blo
     }
 #pragma unroll
     for (int f = 0; f < 8; ++f) {
-      const int m = (grp * 8 + f) * 16 + r;
+      const int m = grp * 128 + r * 8 + f;
       uint16_t b[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float v = acc[f][g][e] + bias[e];
         b[e] = f16 ? __builtin_bit_cast(uint16_t, (_Float16)v) : block_bf16(v);
       }
-      const int u = nq * 16 + g * 4 + q;
-      const int at = (((u >> 1) ^ (m & 7)) << 1) | ((u & 1) ^ ((m >> 3) & 1));
-      *reinterpret_cast<bu32x2*>(smem + m * 512 + at * 8) = bu32x2{b[0] | (uint32_t)b[1] << 16, b[2] | (uint32_t)b[3] << 16};
+      *reinterpret_cast<bu32x2*>(smem + m * 512 + ((nq * 16 + g * 4 + q) ^ (r << 2)) * 8) = bu32x2{b[0] | (uint32_t)b[1] << 16, b[2] | (uint32_t)b[3] << 16};
     }
   }
   __syncthreads();
@@ -210,8 +208,7 @@ __global__ void __launch_bounds__(BlockPP::THREADS) wq_block_pp_kernel(const Blo
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
     const int m = wave * 32 + i * 2 + h, n = n0 + c * 8;
-    bi32x4 x = *reinterpret_cast<const bi32x4*>(smem + m * 512 + ((c ^ (m & 7)) * 16));
-    if ((m >> 3) & 1) x = bi32x4{x[2], x[3], x[0], x[1]};
+    const bi32x4 x = *reinterpret_cast<const bi32x4*>(smem + m * 512 + (c ^ ((m >> 3 & 15) << 1)) * 16);
     if (m0 + m >= a.M || n >= a.N) continue;
     uint16_t* o = reinterpret_cast<uint16_t*>(a.C) + (long)(m0 + m) * a.N + n;
     if (whole) {

@@ -98,7 +98,8 @@ SHAPES = [(1, 1, 16), (1, 16, 128), (1, 129, 144), (2, 300, 1040), (3, 64, 2048)
           (31, 4, 256), (33, 257, 272), (48, 640, 4096), (64, 128, 128), (65, 384, 1024), (100, 1001, 656), (128, 2048, 2048), (130, 256, 6144),
           (9, 7300, 784), (12, 10300, 656), (20, 10250, 1040), (30, 7170, 400), (60, 300, 4112), (64, 6100, 528), (50, 6200, 400),
           (200, 4099, 2064), (256, 512, 384), (300, 130, 4112), (513, 770, 1152), (1000, 1536, 512), (1025, 2050, 1168), (2050, 5000, 272), (3001, 3500, 256), (700, 6000, 272), (513, 9000, 384),
-          (200, 13000, 272), (129, 12800, 384), (129, 12700, 128), (300, 4500, 1040), (190, 8000, 128), (250, 4300, 2064), (256, 4224, 2048)]
+          (200, 13000, 272), (129, 12800, 384), (129, 12700, 128), (300, 4500, 1040), (190, 8000, 128), (250, 4300, 2064), (256, 4224, 2048),
+          (40, 700, 6400), (33, 5000, 4112), (65, 2000, 7184), (100, 5000, 1040), (64, 300, 128), (320, 7600, 256)]
 
 
 @pytest.mark.parametrize("shape", SHAPES, ids=lambda s: "x".join(map(str, s)))
