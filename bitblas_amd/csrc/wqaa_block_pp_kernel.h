@@ -20,6 +20,8 @@
 
 namespace wqaa {
 
+typedef bi32x4 bi32x4_at2 __attribute__((aligned(2)));
+
 struct BlockPP {
   static constexpr int BM = 256, BN = 256, THREADS = 512;
   static constexpr int SLOT = 256 * 128, W_OFF = 3 * SLOT, LDS = 5 * SLOT;
@@ -203,7 +205,6 @@ __global__ void __launch_bounds__(BlockPP::THREADS) wq_block_pp_kernel(const Blo
     }
   }
   __syncthreads();
-  const bool whole = (a.N & 7) == 0;
   const int h = lane >> 5, c = lane & 31;
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
@@ -211,13 +212,12 @@ __global__ void __launch_bounds__(BlockPP::THREADS) wq_block_pp_kernel(const Blo
     const bi32x4 x = *reinterpret_cast<const bi32x4*>(smem + m * 512 + (c ^ ((m >> 3 & 15) << 1)) * 16);
     if (m0 + m >= a.M || n >= a.N) continue;
     uint16_t* o = reinterpret_cast<uint16_t*>(a.C) + (long)(m0 + m) * a.N + n;
-    if (whole) {
-      __builtin_nontemporal_store(x, reinterpret_cast<bi32x4*>(o));
+    if (n + 8 <= a.N) {                                                   // (an odd N puts the piece on any boundary)
+      __builtin_nontemporal_store(x, reinterpret_cast<bi32x4_at2*>(o));
     } else {
-      const int cnt = min(8, a.N - n);
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (e < cnt) o[e] = (uint16_t)((uint32_t)x[e >> 1] >> (16 * (e & 1)));
+      for (int e = 0; e < 7; ++e)
+        if (n + e < a.N) o[e] = (uint16_t)((uint32_t)x[e >> 1] >> (16 * (e & 1)));
     }
   }
 #endif
