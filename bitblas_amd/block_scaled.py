@@ -219,6 +219,7 @@ class BlockScaledMatmul(Operator):
 
     def plan(self, m: int) -> dict:
         """the member a call with `m` rows takes (needs no device)"""
+        self.workspace_bytes(m)
         plan = _lib.Plan()
         _lib.check(_library().wqaa_block_select(self._ref, int(m), ctypes.byref(plan)))
         return plan.as_dict()
@@ -226,6 +227,8 @@ class BlockScaledMatmul(Operator):
     def workspace_bytes(self, m: int) -> int:
         need = self._need.get(m)
         if need is None:
+            if not 0 <= m < 1 << 29:
+                raise ValueError(f"a call takes fewer than 2^29 rows: got {m}")
             need = self._need[m] = int(_library().wqaa_block_workspace_bytes(self._ref, int(m)))
         return need
 
@@ -273,7 +276,7 @@ class BlockScaledMatmul(Operator):
                 self._refuse(A, W, scale_a, scale_w, bias, output)
             bias_ptr = bias.data_ptr()
         if torch.is_grad_enabled():
-            _refuse_grad("BlockScaledMatmul", A, scale_a, scale_w, bias)
+            _refuse_grad("BlockScaledMatmul", A, scale_a, scale_w, bias, output)
         if output is None:
             output = torch.empty(lead + (N,), dtype=self._out, device=A.device)
         elif output.shape != lead + (N,) or output.dtype is not self._out or not output.is_contiguous() or output.get_device() != dev:
@@ -334,7 +337,7 @@ def quantize_blocks(x: torch.Tensor, dtype: str = "e4m3_float8", *, tile: bool =
     if gate is not None and (gate.shape != shape or gate.dtype is not xt or gate.get_device() != dev):
         raise ValueError("gate has the shape, type and device of x")
     if torch.is_grad_enabled():
-        _refuse_grad("quantize_blocks", x, gate)
+        _refuse_grad("quantize_blocks", x, gate, *(output or ()))
     K, lead = shape[-1], shape[:-1]
     m = x.numel() // K
     kb = -(-K // BLOCK)
@@ -453,7 +456,7 @@ def residual_norm(x: torch.Tensor, residual: Optional[torch.Tensor] = None, weig
     if not eps >= 0.0:
         raise ValueError("the norm's eps must be a non-negative number")
     if torch.is_grad_enabled():
-        _refuse_grad("residual_norm", x, residual, weight, post_weight, gate)
+        _refuse_grad("residual_norm", x, residual, weight, post_weight, gate, *(output or ()))
     passes = residual is None and gate is None and post_weight is None and scale == 1.0     # h is x
     if passes and weight is None:
         raise ValueError("nothing to do: no residual, gate, post_weight or scale, and no weight")

@@ -698,6 +698,7 @@ int wqaa_block_matmul(const wqaa_block_desc* desc, const void* A, const void* W,
     set_error(WQAA_ERR_BAD_DESC, "block_matmul: scale_a_ld >= m, and A and W aligned to 16 bytes, are required");
     return WQAA_ERR_BAD_DESC;
   }
+  if (const int bad = block_gemm_check(*desc, m)) return bad;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   StreamDeviceScope scope(s, A);
   if (!device_info().ok) {
@@ -710,12 +711,13 @@ int wqaa_block_matmul(const wqaa_block_desc* desc, const void* A, const void* W,
 }
 
 uint64_t wqaa_block_workspace_bytes(const wqaa_block_desc* desc, int m) {
-  if (!valid_block_desc(desc) || m <= 0) return 0;
+  if (!valid_block_desc(desc) || m <= 0 || block_gemm_check(*desc, m)) return 0;
   return block_gemm_workspace_bytes(*desc, m);
 }
 
 int wqaa_block_select(const wqaa_block_desc* desc, int m, wqaa_plan* plan) {
   if (!valid_block_desc(desc)) return wqaa_last_error();
+  if (const int bad = block_gemm_check(*desc, m <= 0 ? 1 : m)) return bad;
   return block_gemm_plan(*desc, m <= 0 ? 1 : m, plan);
 }
 
@@ -729,6 +731,7 @@ int wqaa_block_quantize(const wqaa_block_quant* q, void* stream) {
     set_error(WQAA_ERR_BAD_DESC, "block_quantize: a null operand, or rows that overlap");
     return WQAA_ERR_BAD_DESC;
   }
+  if (const int bad = block_quantize_check(*q)) return bad;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   StreamDeviceScope scope(s, q->X);
   if (!device_info().ok) {
@@ -751,6 +754,7 @@ int wqaa_residual_norm(const wqaa_residual_norm_args* n, void* stream) {
     set_error(WQAA_ERR_BAD_DESC, "residual_norm: a null operand, nothing to write, or rows that overlap");
     return WQAA_ERR_BAD_DESC;
   }
+  if (const int bad = residual_norm_check(*n)) return bad;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   StreamDeviceScope scope(s, n->x);
   if (!device_info().ok) {

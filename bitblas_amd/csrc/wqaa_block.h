@@ -26,6 +26,10 @@ int block_gemm_plan(const wqaa_block_desc& d, int m, wqaa_plan* plan);
 size_t block_gemm_workspace_bytes(const wqaa_block_desc& d, int m);
 int block_gemm_launch(const wqaa_block_desc& d, const void* A, const void* W, const float* sa, int64_t sa_ld, const float* sw, const void* bias,
                       void* C, int m, void* workspace, uint64_t workspace_bytes, hipStream_t stream);
+// what a launch could not hold, refused before anything touches the device: rows and grids beyond 31 bits, a grid of 2^32 threads
+int block_gemm_check(const wqaa_block_desc& d, int m);
+int block_quantize_check(const wqaa_block_quant& q);
+int residual_norm_check(const wqaa_residual_norm_args& n);
 int block_quantize_launch(const wqaa_block_quant& q, hipStream_t stream);
 int residual_norm_launch(const wqaa_residual_norm_args& n, hipStream_t stream);
 void block_init();

@@ -132,6 +132,19 @@ void block_init() {
   init_pair<1, 1>();
 }
 
+int block_gemm_check(const wqaa_block_desc& d, int m) {
+  constexpr long kThreads = 0xffffffffl;          // of a launch
+  bool ok = m < (1 << 29) && d.N <= 0x7fffffff - 256;                    // (row scales of a block: 31 bits of bytes)
+  if (ok) {
+    const Choice c = choose(d, m);
+    const long wide = c.stream ? c.tiles_n : c.grid();
+    ok = c.tiles() <= 0x3fffffffl && wide * (c.stream ? kStream[c.stream].waves * 64 : c.bm == 256 ? BlockPP::THREADS : c.groups * 256) <= kThreads;
+  }
+  if (ok) return WQAA_OK;
+  set_error(WQAA_ERR_UNSUPPORTED, "block_matmul: m=%d N=%d is too large", m, d.N);
+  return WQAA_ERR_UNSUPPORTED;
+}
+
 size_t block_gemm_workspace_bytes(const wqaa_block_desc& d, int m) {
   const Choice c = choose(d, m);
   return c.split > 1 ? (size_t)c.tiles() * c.split * c.bm * kBlock * 4 : 0;
@@ -160,10 +173,6 @@ int block_gemm_launch(const wqaa_block_desc& d, const void* A, const void* W, co
   if (need && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15))) {
     set_error(WQAA_ERR_BAD_DESC, "block_matmul: m=%d needs %llu bytes of 16-byte aligned workspace", m, (unsigned long long)need);
     return WQAA_ERR_BAD_DESC;
-  }
-  if ((long)c.tiles_m * c.tiles_n > 0x3fffffffl || (int64_t)m * 4 > 0x7fffffff) {
-    set_error(WQAA_ERR_UNSUPPORTED, "block_matmul: m=%d N=%d is too large", m, d.N);
-    return WQAA_ERR_UNSUPPORTED;
   }
   BlockGemmArgs a = {};
   a.A = reinterpret_cast<const unsigned char*>(A), a.W = reinterpret_cast<const unsigned char*>(W);

@@ -371,10 +371,6 @@ int esize(int dt) { return dt == WQAA_F32 ? 4 : 2; }
 
 template <typename K, typename A>
 int launch(K kernel, long grid, int threads, const A& args, hipStream_t stream, const char* what) {
-  if (grid > 0x7fffffffl) {
-    set_error(WQAA_ERR_UNSUPPORTED, "%s: too many rows", what);
-    return WQAA_ERR_UNSUPPORTED;
-  }
   kernel<<<dim3((unsigned)grid), dim3(threads), 0, stream>>>(args);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) {
@@ -384,14 +380,28 @@ int launch(K kernel, long grid, int threads, const A& args, hipStream_t stream, 
   return WQAA_OK;
 }
 
+int too_many(double grid, int threads, const char* what) {               // (double: the product of two 64-bit numbers)
+  if (grid * threads <= 4294967295.0) return WQAA_OK;
+  set_error(WQAA_ERR_UNSUPPORTED, "%s: too many rows for one launch", what);
+  return WQAA_ERR_UNSUPPORTED;
+}
+int norm_vectors(int64_t D) { return (int)((D + 7) / 8) <= 1024 ? 1 : (int)((D + 7) / 8) <= 2048 ? 2 : 4; }     // 8-element pieces of a lane
+int norm_threads(int64_t D) { return (int)(((D + 7) / 8 + norm_vectors(D) - 1) / norm_vectors(D) + 63) / 64 * 64; }
+
 }  // namespace
 
-int block_quantize_launch(const wqaa_block_quant& q, hipStream_t stream) {
+int block_quantize_check(const wqaa_block_quant& q) {
   const bool f16 = q.x_dtype == WQAA_F16, bf16 = q.x_dtype == WQAA_BF16, f32 = q.x_dtype == WQAA_F32;
   if ((!f16 && !bf16 && !f32) || (q.q_dtype != WQAA_E4M3 && q.q_dtype != WQAA_E5M2) || (q.tile && q.gate) || q.K > (1l << 30)) {
     set_error(WQAA_ERR_UNSUPPORTED, "block_quantize: float16 / bfloat16 / float32 to e4m3 / e5m2; a gate goes with rows only");
     return WQAA_ERR_UNSUPPORTED;
   }
+  const double blocks = (double)((q.K + kBlock - 1) / kBlock);
+  return too_many(q.tile ? (double)((q.rows + kBlock - 1) / kBlock) * blocks : (double)((q.rows + 15) / 16) * (double)(((long)blocks + 3) / 4), 256, "block_quantize");
+}
+
+int block_quantize_launch(const wqaa_block_quant& q, hipStream_t stream) {
+  const bool f16 = q.x_dtype == WQAA_F16, bf16 = q.x_dtype == WQAA_BF16;
   QuantArgs a;
   a.x = q.X, a.gate = q.gate, a.q = reinterpret_cast<unsigned char*>(q.Q), a.s = q.S;
   a.rows = q.rows, a.K = q.K, a.x_ld = q.x_ld, a.gate_ld = q.gate_ld, a.s_ld = q.s_ld;
@@ -429,7 +439,7 @@ static int norm_go(const NormArgs& a, int nv, int threads, bool vec, hipStream_t
 #undef WQ_GO
 }
 
-int residual_norm_launch(const wqaa_residual_norm_args& n, hipStream_t stream) {
+int residual_norm_check(const wqaa_residual_norm_args& n) {
   const bool f16 = n.x_dtype == WQAA_F16, bf16 = n.x_dtype == WQAA_BF16;
   auto same_or_f32 = [&](int t) { return t == n.x_dtype || t == WQAA_F32; };
   if ((!f16 && !bf16) || !same_or_f32(n.stream_dtype) || !same_or_f32(n.weight_dtype) || n.D > 32768 ||
@@ -437,15 +447,18 @@ int residual_norm_launch(const wqaa_residual_norm_args& n, hipStream_t stream) {
     set_error(WQAA_ERR_UNSUPPORTED, "residual_norm: float16 / bfloat16 rows of up to 32768, stream and weights of that type or float32");
     return WQAA_ERR_UNSUPPORTED;
   }
+  return too_many((double)n.rows, norm_threads(n.D), "residual_norm");
+}
+
+int residual_norm_launch(const wqaa_residual_norm_args& n, hipStream_t stream) {
+  const bool f16 = n.x_dtype == WQAA_F16;
   NormArgs a;
   a.p = n;
   const int xs = 2, ss = esize(n.stream_dtype);
   const bool vec = n.D % 8 == 0 && aligned(n.x, 16) && n.x_ld * xs % 16 == 0 && (!n.residual || (aligned(n.residual, 16) && n.residual_ld * ss % 16 == 0)) &&
                    (!n.gate || (aligned(n.gate, 16) && n.gate_ld * xs % 16 == 0)) && aligned(n.post_weight, 16) && aligned(n.weight, 16) &&
                    aligned(n.stream, 16) && aligned(n.Y, 16);
-  const int vectors = (int)((n.D + 7) / 8);
-  const int nv = vectors <= 1024 ? 1 : vectors <= 2048 ? 2 : 4;
-  const int threads = ((vectors + nv - 1) / nv + 63) / 64 * 64;
+  const int nv = norm_vectors(n.D), threads = norm_threads(n.D);
   if (f16) return n.stream_dtype == WQAA_F32 ? norm_go<WQAA_F16, true>(a, nv, threads, vec, stream) : norm_go<WQAA_F16, false>(a, nv, threads, vec, stream);
   return n.stream_dtype == WQAA_F32 ? norm_go<WQAA_BF16, true>(a, nv, threads, vec, stream) : norm_go<WQAA_BF16, false>(a, nv, threads, vec, stream);
 }

@@ -170,3 +170,42 @@ def test_scale_layouts():
     assert ld == 1 and one.shape == (1, 5)
     wide = torch.empty(5, 9).t()[:6]                                     # rows of a block side by side, blocks further apart
     assert bs._scale_rows(wide, 6, 5)[1] == 9
+
+
+def test_more_rows_than_a_launch_holds():
+    """row counts whose bytes, grid or threads leave 32 bits: refused on the host, at both boundaries"""
+    L = bs._library()
+    p = 4096
+
+    def product(m, **kw):
+        return L.wqaa_block_matmul(ctypes.byref(_desc(**kw)), p, p, p, m, p, None, p, m, p, 1 << 60, None)
+
+    for m in (1 << 29, (1 << 31) - 1):
+        assert product(m) == wlib.ERR_UNSUPPORTED
+        assert L.wqaa_block_workspace_bytes(ctypes.byref(_desc()), m) == 0
+        assert L.wqaa_block_select(ctypes.byref(_desc()), m, None) == wlib.ERR_UNSUPPORTED
+    assert product(1, N=(1 << 31) - 1, K=16) == wlib.ERR_UNSUPPORTED      # 2^27 workgroups of 512 threads
+    assert L.wqaa_block_select(ctypes.byref(_desc(N=1 << 20)), (1 << 29) - 1, None) == wlib.ERR_UNSUPPORTED
+    op = bitblas.BlockScaledMatmul(bitblas.BlockScaledMatmulConfig(N=256, K=256))
+    assert op.plan((1 << 29) - 1)["grid"] > 0
+    for m in (1 << 29, 1 << 32, -1):                                      # (2^32: nothing of it may be cut off on the way)
+        with pytest.raises(ValueError):
+            op.plan(m)
+        with pytest.raises(ValueError):
+            op.workspace_bytes(m)
+
+    a = bs.BlockQuant(bs._QUANT_BYTES, wlib.BF16, wlib.E4M3, 0, 1 << 28, 1, 1, 1, 1 << 28, p, None, p, p)
+    a.rows = (1 << 28) + 16                                               # 2^24 + 1 workgroups of 256 threads
+    a.s_ld = a.rows
+    assert L.wqaa_block_quantize(ctypes.byref(a), None) == wlib.ERR_UNSUPPORTED
+    a.rows = (1 << 62) + 1
+    a.s_ld = a.rows
+    assert L.wqaa_block_quantize(ctypes.byref(a), None) == wlib.ERR_UNSUPPORTED
+    n = bs.ResidualNormArgs(bs._NORM_BYTES, wlib.BF16, wlib.BF16, wlib.BF16, -1, 1e-5, 1.0, 1.0, 1 << 26, 16, 16)
+    n.x = n.weight = n.Y = p
+    assert L.wqaa_residual_norm(ctypes.byref(n), None) == wlib.ERR_UNSUPPORTED
+
+
+def test_outputs_that_autograd_tracks_are_refused():
+    with pytest.raises(RuntimeError, match="no backward"):
+        bs._refuse_grad("residual_norm", torch.zeros(2), None, torch.zeros(2, requires_grad=True))

@@ -621,3 +621,63 @@ def test_product_repeats_bit_for_bit(M):
     first = op(A, W, sa, sw)
     for _ in range(5):
         assert torch.equal(op(A, W, sa, sw), first)
+
+
+def _inside(room, at, shape):
+    """a contiguous view into `room`, and what lies around it"""
+    n = 1
+    for size in shape:
+        n *= size
+    return room[at:at + n].view(shape), torch.cat([room[:at], room[at + n:]])
+
+
+@pytest.mark.parametrize("M, N, K", [(5, 131, 272), (40, 1001, 272), (70, 6101, 144), (70, 301, 7184), (260, 9001, 144), (600, 6301, 144), (1281, 8713, 144)])
+def test_product_odd_columns(M, N, K):
+    """N odd, so every row starts on another boundary, and an output that starts off any: right, and nothing written beside it"""
+    A, W, sa, sw = operands(M, N, K, seed=N)
+    op = bitblas.BlockScaledMatmul(bitblas.BlockScaledMatmulConfig(N=N, K=K, out_dtype="bfloat16"))
+    dev = [t.cuda() for t in (A, W, sa, sw)]
+    room = torch.full((M * N + 64,), 7.0, dtype=torch.bfloat16, device="cuda")
+    out, around = _inside(room, 17, (M, N))
+    op(*dev, output=out)
+    out, around = _inside(room, 17, (M, N))
+    assert bool((around == 7.0).all())
+    assert torch.equal(out, op(*dev))
+    check_product(out, A, W, sa, sw)
+
+
+@pytest.mark.parametrize("K", [1, 9, 127, 1041, 4095, 8193])
+@pytest.mark.parametrize("x", list(TO))
+def test_odd_rows_beside_others(K, x):
+    """quantiser and norm over rows of an odd width, inputs and outputs on odd boundaries: the same bits as anywhere, nothing beside them"""
+    m, q8 = 37, "e4m3_float8"
+    wide = torch.randn(m * K + 64, generator=gen(K)).to(TO[x]).cuda()
+    src, gate = wide[5:5 + m * K].view(m, K), wide[3:3 + m * K].view(m, K)
+    for kw in (dict(), dict(tile=True), dict(gate=gate)):
+        want = bitblas.quantize_blocks(src.clone(), q8, **{k: v.clone() if k == "gate" else v for k, v in kw.items()})
+        room = torch.full((m * K + 64,), 1.0, device="cuda").to(torch.float8_e4m3fn)
+        out, _ = _inside(room, 9, (m, K))
+        q, s = bitblas.quantize_blocks(src, q8, output=(out, torch.empty_like(want[1])), **kw)
+        assert torch.equal(q.view(torch.uint8), want[0].view(torch.uint8)) and torch.equal(s, want[1])
+        assert bool((_inside(room, 9, (m, K))[1].float() == 1.0).all())
+    if x == "float32":
+        return
+    w = torch.randn(K + 1, generator=gen(K + 1)).to(TO[x]).cuda()
+    for st in (TO[x], torch.float32):
+        res = torch.randn(m * K + 8, generator=gen(K + 2)).to(st).cuda()[3:3 + m * K].view(m, K)
+        want = bitblas.residual_norm(src.clone(), res.clone(), w[1:].clone(), 1e-5, gate=gate.clone())
+        h_room, y_room = torch.full((m * K + 64,), 7.0, dtype=st, device="cuda"), torch.full((m * K + 64,), 7.0, dtype=TO[x], device="cuda")
+        bitblas.residual_norm(src, res, w[1:], 1e-5, gate=gate, output=(_inside(h_room, 11, (m, K))[0], _inside(y_room, 13, (m, K))[0]))
+        for room, at, have in ((h_room, 11, want[0]), (y_room, 13, want[1])):
+            out, around = _inside(room, at, (m, K))
+            assert torch.equal(out, have) and bool((around == 7.0).all())
+
+
+def test_outputs_that_autograd_tracks():
+    A, W, sa, sw = [t.cuda() for t in operands(4, 32, 128)]
+    op = bitblas.BlockScaledMatmul(bitblas.BlockScaledMatmulConfig(N=32, K=128))
+    with pytest.raises(RuntimeError, match="no backward"):
+        op(A, W, sa, sw, output=torch.zeros(4, 32, dtype=torch.float16, device="cuda", requires_grad=True))
+    x = torch.zeros(4, 128, dtype=torch.float16, device="cuda")
+    with pytest.raises(RuntimeError, match="no backward"):
+        bitblas.residual_norm(x, x, output=(torch.zeros_like(x, requires_grad=True),))
