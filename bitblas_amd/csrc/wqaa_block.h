@@ -13,12 +13,13 @@ struct BlockGemmArgs {
   const float* sw;                           // scale of (tile t, block b) at sw[t * KB + b]
   const void* bias;                          // (N,) of the output type, or null
   void* C;                                   // (M, N)
-  float* ws;                                 // partial tiles of the K slices: (tile, slice, BM, 128)
+  float* ws;                                 // partial tiles of the K slices: (tile behind the whole ones, slice, BM, BN)
   long sa_ld;
   int M, N, K, KB;                           // KB = ceil(K / 128)
   int out_dtype;                             // wqaa_dtype
   int tiles_m, tiles_n;
-  int split, split_len;                      // workgroups of a tile: slice z takes k-blocks [z * split_len, min(KB, (z + 1) * split_len))
+  // the first `whole` tiles have a workgroup each; the others `split`, slice z of them k-blocks [z * split_len, min(KB, (z + 1) * split_len))
+  int whole, split, split_len;
   int group_m;                               // M-tiles that share an N-tile back to back
 };
 

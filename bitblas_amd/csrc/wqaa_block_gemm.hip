@@ -10,9 +10,10 @@ struct Choice {
   int stream;            // > 0: the streaming member, which form of it (kStream, launch_pair)
   int bm;                // tile members: activation rows of a tile (256: the ping-pong member, whose tiles are 256 weight rows wide)
   int groups;            // tile member: groups of four waves in a workgroup (BlockTile::G)
-  int tiles_m, tiles_n, split, split_len;
+  int tiles_m, tiles_n, whole, split, split_len;      // whole: tiles with a workgroup each; the others have `split`
   long tiles() const { return (long)tiles_m * tiles_n; }
-  long grid() const { return tiles() * split; }
+  long grid() const { return whole + (tiles() - whole) * split; }
+  int bn() const { return bm == 256 ? 256 : kBlock; }
 };
 
 Choice choose(const wqaa_block_desc& d, int m) {
@@ -40,19 +41,45 @@ Choice choose(const wqaa_block_desc& d, int m) {
   if (m <= 32 || (rounds2 <= 2 && rounds2 * kb <= 32)) return stream(6, 32, 2);
   auto tiles_of = [&](int bm, int bn) {
     c.bm = bm, c.tiles_m = (m + bm - 1) / bm, c.tiles_n = (d.N + bn - 1) / bn;
-    c.split = 1, c.split_len = kb;
-    return (long)c.tiles_m * c.tiles_n;
+    c.split = 1, c.split_len = kb, c.whole = (int)c.tiles();
+    return c.tiles();
   };
-  // many rows: the ping-pong member, where its 256 x 256 tiles (one a CU) leave less than about a third of their last round empty:
-  // 1024 x 11008 x 4096, 172 tiles, 66 us against 69 for 128-row tiles; 4096 x 5120 x 5120, 320 tiles, 131 against 125;
-  // 2048 x 11008 x 4096, 344 tiles, 109 against 113; 2048 x 28672 x 8192, 896 tiles, 435 against 517
-  const long big = tiles_of(256, 256), rounds = (big + 255) / 256;
-  if (m > 128 && big * 20 >= rounds * 256 * 13) return c;
+  auto slices = [&](long whole, long split) {    // the tiles behind the first `whole` of them in K slices
+    c.split_len = (int)((kb + split - 1) / split);
+    c.split = (kb + c.split_len - 1) / c.split_len;
+    if (c.split > 1) c.whole = (int)whole;
+  };
+  // many rows: the ping-pong member, a 256 x 256 tile per CU at a time.  The tiles of a last round that is not full may leave in K slices, so
+  // that it takes a half to a quarter of a round: saves 1.5 us for every k-block it is shorter, costs 0.09 us for every partial tile, to
+  // memory and back, and 6 us for the launch that adds them: 4096 x 4352 x 4096, 272 tiles, 112 us whole, 98 with the last 16 in 2
+  // slices, 91 in 4, 94 in 7; 4096 x 5120 x 5120, 320 tiles, 141, 136 and 126 in 4; 3000 x 8192 x 8192, 384 tiles, 236 and 223 in 2; 4096 x
+  // 9472 x 2048, 592 tiles, 115, 117 in 2, 134 in 4
+  const long big = tiles_of(256, 256), rounds = (big + 255) / 256, rest = big % 256;
+  if (big > 0x3fffffffl) return c;                // (block_gemm_check refuses it)
+  long split = 1, saved = 0;                      // units of 0.1 us
+  for (long z = 2; z <= 4 && rounds > 1 && rest * z <= 256; ++z) {
+    const long gain = 15 * (kb - (kb + z - 1) / z) - rest * z * 9 / 10 - 60;
+    if (rest > 0 && gain > saved) split = z, saved = gain;
+  }
+  // taken where less than about a third of the time of its rounds is lost: 1024 x 11008 x 4096, 172 tiles, 66 us against 69 for 128-row tiles;
+  // 2048 x 10240 x 4096, 320 tiles, the last 64 in 4 slices, 110 (114 whole) against 125; 2048 x 28672 x 8192, 896 tiles, 435 against 517
+  if (m > 128 && big * 20 * 15 * kb >= 13 * 256 * (15 * kb * rounds - saved)) {
+    if (split > 1) slices(big - rest, split);
+    return c;
+  }
   // tiles of 128 rows where they are a tile per CU or nearly, or more than two of 64 rows per CU: 512 x 8192 x 8192, 256 of them, 43 us
   // against 50 for 512 of 64 rows; 128 x 28672 x 8192, 224 of them, 65 against 70; 700 x 8192 x 4096, 704 of 64 rows, 36 against 41
   const long t128 = tiles_of(128, kBlock);
   const bool one_each = t128 >= 192 && t128 <= 256;
   const long t64 = (long)((m + 63) / 64) * c.tiles_n;
+  // 64 rows, two of them a CU, and little more than a round: that in 4 slices (333 x 11008 x 4096, 516 tiles, 35.3 us against 39.5 for 258 of 128
+  // rows; 512 x 9216 x 8192, 576 tiles, 65.3 against 67.9; 640 x 8192 x 2048, 640 tiles, 30 against 25)
+  if (m > 64 && t64 > 512 && t64 <= 512 + 64 && kb >= 32) {
+    (void)tiles_of(64, kBlock);
+    c.groups = 1;
+    slices(512, 4);
+    return c;
+  }
   if (m > 64 && (one_each || t64 > 512)) {
     c.groups = one_each ? 2 : 1;
     return c;
@@ -64,13 +91,10 @@ Choice choose(const wqaa_block_desc& d, int m) {
   // 19.7 us, 4 slices of one 21.2; 512 x 1024 x 4096, 64 tiles, 4 slices 13.8 us, none 20
   c.groups = t64 >= 128 && t64 <= 256 ? 2 : 1;
   if (t64 < 160) {
-    long split = c.groups == 2 ? 2 : 256 / t64;
-    if (split > 8) split = 8;
-    if (split > kb / 4) split = kb / 4;
-    if (split > 1) {
-      c.split_len = (int)((kb + split - 1) / split);
-      c.split = (kb + c.split_len - 1) / c.split_len;
-    }
+    long z = c.groups == 2 ? 2 : 256 / t64;
+    if (z > 8) z = 8;
+    if (z > kb / 4) z = kb / 4;
+    if (z > 1) slices(0, z);
   }
   return c;
 }
@@ -119,8 +143,8 @@ void launch_pair(const Choice& c, const BlockGemmArgs& a, hipStream_t s) {
   else if (c.bm == 64) tail ? tile_go<BlockTile<WF, AF, 64, 3, 1, true>>(c, a, s) : tile_go<BlockTile<WF, AF, 64, 3, 1, false>>(c, a, s);
   else if (c.bm == 128 && c.groups == 2) tail ? tile_go<BlockTile<WF, AF, 128, 2, 2, true>>(c, a, s) : tile_go<BlockTile<WF, AF, 128, 2, 2, false>>(c, a, s);
   else if (c.bm == 128) tail ? tile_go<BlockTile<WF, AF, 128, 2, 1, true>>(c, a, s) : tile_go<BlockTile<WF, AF, 128, 2, 1, false>>(c, a, s);
-  else if (tail) wq_block_pp_kernel<WF, AF, true><<<dim3(a.tiles_m * a.tiles_n), dim3(BlockPP::THREADS), BlockPP::LDS, s>>>(a);
-  else wq_block_pp_kernel<WF, AF, false><<<dim3(a.tiles_m * a.tiles_n), dim3(BlockPP::THREADS), BlockPP::LDS, s>>>(a);
+  else if (tail) wq_block_pp_kernel<WF, AF, true><<<dim3((unsigned)c.grid()), dim3(BlockPP::THREADS), BlockPP::LDS, s>>>(a);
+  else wq_block_pp_kernel<WF, AF, false><<<dim3((unsigned)c.grid()), dim3(BlockPP::THREADS), BlockPP::LDS, s>>>(a);
 }
 
 }  // namespace
@@ -147,7 +171,7 @@ int block_gemm_check(const wqaa_block_desc& d, int m) {
 
 size_t block_gemm_workspace_bytes(const wqaa_block_desc& d, int m) {
   const Choice c = choose(d, m);
-  return c.split > 1 ? (size_t)c.tiles() * c.split * c.bm * kBlock * 4 : 0;
+  return c.split > 1 ? (size_t)(c.tiles() - c.whole) * c.split * c.bm * c.bn() * 4 : 0;
 }
 
 int block_gemm_plan(const wqaa_block_desc& d, int m, wqaa_plan* plan) {
@@ -181,14 +205,18 @@ int block_gemm_launch(const wqaa_block_desc& d, const void* A, const void* W, co
   a.C = C, a.ws = reinterpret_cast<float*>(workspace);
   a.M = m, a.N = d.N, a.K = d.K, a.KB = (d.K + kBlock - 1) / kBlock;
   a.out_dtype = d.out_dtype;
-  a.tiles_m = c.tiles_m, a.tiles_n = c.tiles_n, a.split = c.split, a.split_len = c.split_len;
+  a.tiles_m = c.tiles_m, a.tiles_n = c.tiles_n, a.whole = c.whole, a.split = c.split, a.split_len = c.split_len;
   a.group_m = c.tiles_m < 8 ? c.tiles_m : 8;
   const int wf = d.w_dtype == WQAA_E5M2, af = d.a_dtype == WQAA_E5M2;
   if (wf == 0 && af == 0) launch_pair<0, 0>(c, a, stream);
   else if (wf == 0) launch_pair<0, 1>(c, a, stream);
   else if (af == 0) launch_pair<1, 0>(c, a, stream);
   else launch_pair<1, 1>(c, a, stream);
-  if (c.split > 1) wq_block_reduce_kernel<<<dim3((unsigned)(c.tiles() * (c.bm / 8))), dim3(256), 0, stream>>>(a, c.bm);
+  if (c.split > 1) {
+    const dim3 g((unsigned)((c.tiles() - c.whole) * (c.bm * c.bn() / 1024)));
+    if (c.bm == 256) wq_block_reduce_kernel<256><<<g, dim3(256), 0, stream>>>(a, c.bm);
+    else wq_block_reduce_kernel<kBlock><<<g, dim3(256), 0, stream>>>(a, c.bm);
+  }
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) {
     set_error(WQAA_ERR_LAUNCH, "block_matmul: %s", hipGetErrorString(e));

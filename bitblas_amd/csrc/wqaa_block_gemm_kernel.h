@@ -61,8 +61,9 @@ __device__ __forceinline__ void block_store4(void* C, int dt, long i, int n, con
 // One read of W is nearly all there is to do, so nothing is staged: a wave takes NF fragments of 16 weight rows and every WAVES-th
 // k-block of them straight into the matrix operand's registers (two 16-byte loads a lane and fragment), the MF fragments of activation rows -
 // from L2 - the same way; the waves' partial tiles meet in LDS in a fixed order.  Rows beyond m and n repeat the last one and are
-// not stored.  Workgroups along y take 16 MF rows each.  U blocks are asked for at once; PF: the next U before the matrix instructions of these.  NF > 1 divides the reads of the
-// activations, which at 16 rows are as many as those of the weights (choose() in wqaa_block_gemm.hip has the measured rule).
+// not stored.  Workgroups along y take 16 MF rows each.  U blocks are asked for at once; PF: the next U before the matrix
+// instructions of these.  NF > 1 divides the reads of the activations, which at 16 rows are as many as those of the weights (choose() in
+// wqaa_block_gemm.hip has the measured rule).  One row, 28672 x 8192: 38.6 us, 6.1 TB/s; 16 rows, 8192 x 28672: 46 us, 5.1 TB/s.
 template <int WF, int AF, int WAVES, int U, int NF, int MF, bool PF>
 __global__ void __launch_bounds__(WAVES * 64) wq_block_stream_kernel(const BlockGemmArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -209,7 +210,8 @@ __global__ void __launch_bounds__(WAVES * 64) wq_block_stream_kernel(const Block
 //   G = 2  two such groups of four waves in ONE workgroup, each with its half of the k-blocks and its own ring, one barrier apart: while
 //          one reads operands and issues copies (load phase), the other multiplies.  Their sums meet in LDS at the end.  For grids
 //          of up to a tile per CU.
-// split > 1: that many workgroups take a K slice of the tile each and leave float32 partial tiles for the reduce launch behind this one.
+// split > 1: the tiles behind the first `whole` have that many workgroups, each with a K slice, which leave float32 partial tiles for the
+// reduce launch behind this one: all tiles of a grid that would not fill the chip, or what is left over from its whole rounds.
 // TAIL: K is no multiple of 128 (pieces of the last block beyond K are fetched from outside the buffer, which reads as zero)
 template <int WF_, int AF_, int BM_, int S_, int G_, bool TAIL_>
 struct BlockTile {
@@ -240,9 +242,8 @@ __device__ __forceinline__ void block_wait_vm() {
     asm volatile("" ::: "memory");          \
   } while (0)
 
-// tile `blk` of `nblk`: an XCD's workgroups (index modulo 8) walk neighbouring tiles, group_m M-tiles for each N-tile
-__device__ __forceinline__ void block_tile_of(const BlockGemmArgs& a, int blk, int nblk, int& tile_m, int& tile_n) {
-  if ((nblk & 7) == 0) blk = (blk & 7) * (nblk >> 3) + (blk >> 3);
+// tile `t` in the order of the walk: group_m M-tiles for each N-tile
+__device__ __forceinline__ void block_tile_at(const BlockGemmArgs& a, int blk, int& tile_m, int& tile_n) {
   const int per_group = a.group_m * a.tiles_n;
   const int group = blk / per_group;
   const int first_m = group * a.group_m;
@@ -250,6 +251,25 @@ __device__ __forceinline__ void block_tile_of(const BlockGemmArgs& a, int blk, i
   const int rem = blk - group * per_group;
   tile_m = first_m + rem % gsz;
   tile_n = rem / gsz;
+}
+// what this workgroup takes: a tile, and which k-blocks of it.  An XCD's workgroups (index modulo 8) walk neighbouring tiles.
+struct BlockShare {
+  int tile_m, tile_n, first, end;            // k-blocks first ... end - 1
+  long part;                                 // the partial tile that it leaves, or -1: the tile is its own
+};
+__device__ __forceinline__ BlockShare block_share(const BlockGemmArgs& a) {
+  auto walk = [](int i, int n) { return (n & 7) == 0 ? (i & 7) * (n >> 3) + (i >> 3) : i; };
+  BlockShare w;
+  const int blk = blockIdx.x;
+  if (blk < a.whole) {
+    block_tile_at(a, walk(blk, a.whole), w.tile_m, w.tile_n);
+    w.first = 0, w.end = a.KB, w.part = -1;
+  } else {
+    const int i = blk - a.whole, t = i / a.split, z = i - t * a.split;
+    block_tile_at(a, a.whole + walk(t, a.tiles_m * a.tiles_n - a.whole), w.tile_m, w.tile_n);
+    w.first = z * a.split_len, w.end = min(a.KB, w.first + a.split_len), w.part = i;
+  }
+  return w;
 }
 
 template <class P>
@@ -262,10 +282,8 @@ __global__ void __launch_bounds__(P::THREADS, 2 / P::G) wq_block_tile_kernel(con
   const int r = lane & 15, q = lane >> 4;
   const int wm = wave / P::WN, wn = wave % P::WN;
 
-  int tile_m, tile_n;
-  const int tile = blockIdx.x / a.split, slice = blockIdx.x - tile * a.split;
-  block_tile_of(a, tile, a.tiles_m * a.tiles_n, tile_m, tile_n);
-  const int s_first = slice * a.split_len, s_end = min(a.KB, s_first + a.split_len);
+  const BlockShare share = block_share(a);
+  const int tile_m = share.tile_m, tile_n = share.tile_n, s_first = share.first, s_end = share.end;
   // this group's k-blocks: b_first ... b_first + mine - 1; both groups take nt steps
   const int nt = (s_end - s_first + P::G - 1) / P::G;
   const int b_first = s_first + grp * nt, mine = min(nt, s_end - b_first);
@@ -413,8 +431,8 @@ __global__ void __launch_bounds__(P::THREADS, 2 / P::G) wq_block_tile_kernel(con
 #pragma unroll
     for (int g = 0; g < P::NF; ++g) {
       const int nl = (wn * P::NF + g) * 16 + q * 4, n = n0 + nl;
-      if (a.split > 1) {                          // a slice: the whole tile, rows and columns beyond the matrix included
-        *reinterpret_cast<bf32x4*>(a.ws + (((long)tile * a.split + slice) * P::BM + ml) * P::BN + nl) = acc[f][g];
+      if (share.part >= 0) {                      // a slice: the whole tile, rows and columns beyond the matrix included
+        *reinterpret_cast<bf32x4*>(a.ws + (share.part * P::BM + ml) * P::BN + nl) = acc[f][g];
         continue;
       }
       if (m >= a.M || n >= a.N) continue;
@@ -428,18 +446,20 @@ __global__ void __launch_bounds__(P::THREADS, 2 / P::G) wq_block_tile_kernel(con
 #endif
 }
 
-// partial tiles of the K slices, in slice order: a workgroup takes 256 x 4 elements of a tile (tile rows of 128, so 8 rows)
+// partial tiles of the K slices, in slice order: a workgroup takes 256 x 4 elements of a tile
+template <int BN>
 __global__ void __launch_bounds__(256) wq_block_reduce_kernel(const BlockGemmArgs a, int bm) {
-  const int per_tile = bm / 8;
-  const int t = blockIdx.x / per_tile, part = blockIdx.x % per_tile;
+  constexpr int LANES = BN / 4, ROWS = 256 / LANES;
+  const int per_tile = bm / ROWS;
+  const int t = blockIdx.x / per_tile, part = blockIdx.x % per_tile, left = a.tiles_m * a.tiles_n - a.whole;
   int tile_m, tile_n;
-  block_tile_of(a, t, a.tiles_m * a.tiles_n, tile_m, tile_n);
-  const int ml = part * 8 + (threadIdx.x >> 5), nl = (threadIdx.x & 31) * 4;
-  const int m = tile_m * bm + ml, n = tile_n * kBlock + nl;
+  block_tile_at(a, a.whole + ((left & 7) == 0 ? (t & 7) * (left >> 3) + (t >> 3) : t), tile_m, tile_n);
+  const int ml = part * ROWS + threadIdx.x / LANES, nl = threadIdx.x % LANES * 4;
+  const int m = tile_m * bm + ml, n = tile_n * BN + nl;
   if (m >= a.M || n >= a.N) return;
-  const float* p = a.ws + ((long)t * a.split * bm + ml) * kBlock + nl;
+  const float* p = a.ws + ((long)t * a.split * bm + ml) * BN + nl;
   bf32x4 v = {0.f, 0.f, 0.f, 0.f};
-  for (int z = 0; z < a.split; ++z) v += *reinterpret_cast<const bf32x4*>(p + (long)z * bm * kBlock);
+  for (int z = 0; z < a.split; ++z) v += *reinterpret_cast<const bf32x4*>(p + (long)z * bm * BN);
   const int cnt = min(4, a.N - n);
   float o[4];
 #pragma unroll

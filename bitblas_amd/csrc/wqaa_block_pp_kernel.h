@@ -39,19 +39,18 @@ __global__ void __launch_bounds__(BlockPP::THREADS) wq_block_pp_kernel(const Blo
   const int grp = wave >> 2, nq = wave & 3;
   const int r = lane & 15, q = lane >> 4;
 
-  int tile_m, tile_n;
-  block_tile_of(a, blockIdx.x, gridDim.x, tile_m, tile_n);
-  const int m0 = tile_m * P::BM, n0 = tile_n * P::BN;
-  const int nt = a.KB;
+  const BlockShare share = block_share(a);
+  const int m0 = share.tile_m * P::BM, n0 = share.tile_n * P::BN;
+  const int nt = share.end - share.first, k0 = share.first * kBlock;     // a slice: everything below starts at its first block
 
-  const long a_bytes = (long)min(P::BM, a.M - m0) * a.K, w_bytes = (long)min(P::BN, a.N - n0) * a.K;
-  const auto a_rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(a.A + (long)m0 * a.K), 0, (int)a_bytes, 0x00020000);
-  const auto w_rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(a.W + (long)n0 * a.K), 0, (int)w_bytes, 0x00020000);
+  const long a_bytes = (long)min(P::BM, a.M - m0) * a.K - k0, w_bytes = (long)min(P::BN, a.N - n0) * a.K - k0;
+  const auto a_rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(a.A + (long)m0 * a.K + k0), 0, (int)a_bytes, 0x00020000);
+  const auto w_rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(a.W + (long)n0 * a.K + k0), 0, (int)w_bytes, 0x00020000);
   constexpr uint32_t OUT = 0xC0000000u;
   const int g0 = (lane & 7) ^ ((lane >> 4) & 7);
   // first row of the wave's pieces: W's rows in order, A's as LDS rows 32 wave + 8 j + lane / 8 hold them (j & 1: 64 rows on, j / 2: one)
   const uint32_t w_row = wave * 32 + (lane >> 3), a_row = grp * 128 + (lane >> 3) * 8 + nq * 2;
-  const int tail = a.K - (nt - 1) * kBlock;
+  const int tail = a.K - k0 - (nt - 1) * kBlock;                          // (a slice that is not the last: more than a block)
   const bool cut0 = TAIL && g0 * 16 >= tail, cut1 = TAIL && (g0 ^ 4) * 16 >= tail;
 
   auto piece = [&](const auto& rsrc, uint32_t row, unsigned char* dst, int tt, int j) {
@@ -66,12 +65,12 @@ __global__ void __launch_bounds__(BlockPP::THREADS) wq_block_pp_kernel(const Blo
   const uint32_t srow = (uint32_t)(m0 + grp * 128 + r * 8) * 4u;
   bf32x4 raw[2];
   auto fetch_scales = [&](int tt) {                                       // rows beyond M are outside the buffer: zero
-    const auto rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(a.sa + (long)min(tt, nt - 1) * a.sa_ld), 0, a.M * 4, 0x00020000);
+    const auto rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(a.sa + (long)(share.first + min(tt, nt - 1)) * a.sa_ld), 0, a.M * 4, 0x00020000);
     raw[0] = __builtin_bit_cast(bf32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, srow, 0, 0));
     raw[1] = __builtin_bit_cast(bf32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, srow + 16u, 0, 0));
   };
   const int nb = min((n0 + nq * 64) / kBlock, (a.N - 1) / kBlock);
-  const auto* swp = (const __attribute__((address_space(4))) float*)(a.sw + (long)nb * nt);
+  const auto* swp = (const __attribute__((address_space(4))) float*)(a.sw + (long)nb * a.KB + share.first);
 
   const int swl = (r >> 1) & 7;
   const int rd0 = r * 128 + ((q ^ swl) * 16), rd1 = r * 128 + (((4 + q) ^ swl) * 16);
@@ -181,6 +180,14 @@ __global__ void __launch_bounds__(BlockPP::THREADS) wq_block_pp_kernel(const Blo
   block_wait_vm<0>();                                                     // no copy may land in what the epilogue stages
   WQ_BLOCK_BARRIER();
 
+  if (share.part >= 0) {                                                  // a slice: the whole tile, rows and columns beyond the matrix included
+    float* const o = a.ws + share.part * (P::BM * P::BN) + (grp * 128 + r * 8) * P::BN + nq * 64 + q * 4;
+#pragma unroll
+    for (int f = 0; f < 8; ++f)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) *reinterpret_cast<bf32x4*>(o + f * P::BN + g * 16) = acc[f][g];
+    return;
+  }
   // the tile leaves through LDS, whole rows per store: row m at 512 m, its 8-byte unit u (four n) at u ^ 4 (m / 8 mod 16) - the 64
   // lanes of a write, 16 rows 8 apart, then meet every bank twice, and 16-byte pieces stay whole
   const bool f16 = a.out_dtype == WQAA_F16;

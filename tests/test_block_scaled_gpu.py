@@ -681,3 +681,21 @@ def test_outputs_that_autograd_tracks():
     x = torch.zeros(4, 128, dtype=torch.float16, device="cuda")
     with pytest.raises(RuntimeError, match="no backward"):
         bitblas.residual_norm(x, x, output=(torch.zeros_like(x, requires_grad=True),))
+
+
+@pytest.mark.parametrize("M, N, K", [(257, 32900, 4112), (4300, 4001, 4096), (70, 32851, 4112)])
+def test_product_last_round_in_slices(M, N, K):
+    """whole tiles, and behind them some in K slices: right, the same every time, and nothing written beside the output"""
+    A, W, sa, sw = operands(M, N, K, seed=N)
+    bias = torch.randn(N, generator=gen(N)).bfloat16()
+    op = bitblas.BlockScaledMatmul(bitblas.BlockScaledMatmulConfig(N=N, K=K, out_dtype="bfloat16", with_bias=True))
+    plan = op.plan(M)
+    tiles = -(-M // plan["block_m"]) * -(-N // plan["block_n"])
+    assert plan["split_k"] > 1 and tiles < plan["grid"] < tiles * plan["split_k"]
+    dev = [t.cuda() for t in (A, W, sa, sw, bias)]
+    room = torch.full((M + 2, N), 7.0, dtype=torch.bfloat16, device="cuda")
+    first = op(*dev, output=room[1:M + 1])
+    assert bool((room[0] == 7.0).all()) and bool((room[M + 1] == 7.0).all())
+    check_product(first, A, W, sa, sw, bias)
+    for _ in range(3):
+        assert torch.equal(op(*dev), first)
