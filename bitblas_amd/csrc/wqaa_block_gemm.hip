@@ -32,13 +32,14 @@ Choice choose(const wqaa_block_desc& d, int m) {
   if (m <= 16) return m > 4 && d.N >= 10240 ? stream(4, 16, 4) : m > 4 && d.N >= 7168 ? stream(3, 16, 2) : kb >= 64 ? stream(2, 16, 1) : stream(1, 16, 1);
   // 32 rows a workgroup, more of them along y: small products are through before tiles and their partial sums would be.  One fragment
   // while that is about a workgroup per CU (77 x 1001 x 1040 3.2 us against 3.8 with two and 8.4 for tiles; 128 x 1024 x 4096 7.7, 9.7 and
-  // 11.1), else two while they take a round of the chip, or two on short K (64 x 4096 x 4096 10.0 us against 13.7 for tiles, 64 x 6144 x 4096
-  // 17.2 against 13.4; 256 x 2048 x 2048 10.0 against 12.0).  Up to 32 rows there is nothing W could be shared with: 24 x 6144 x 4096 9.5 us
+  // 11.1), else two while they take a round of the chip, or up to four on short K (64 x 4096 x 4096 10.0 us against 13.7 for tiles, 64 x 6144 x 4096
+  // 17.2 against 13.4; 256 x 2048 x 2048 10.0 against 12.0; 333 x 2048 x 1024, three rounds, 8.6 against 11.1;
+  // 600 x 1024 x 2048 13.6 against 12.6).  Up to 32 rows there is nothing W could be shared with: 24 x 6144 x 4096 9.5 us
   // with two, 12.0 with one; 32 x 11008 x 4096 14.6 us with four, 17.2 with two.
   const long chunks = (m + 31) / 32, one = chunks * ((d.N + 15) / 16), two = chunks * ((d.N + 31) / 32), rounds2 = (two + 255) / 256;
   if (one <= 288 && (m <= 32 || kb <= 48)) return stream(5, 32, 1);
   if (m <= 32 && d.N >= 10240) return stream(7, 32, 4);
-  if (m <= 32 || (rounds2 <= 2 && rounds2 * kb <= 32)) return stream(6, 32, 2);
+  if (m <= 32 || (rounds2 <= 4 && rounds2 * kb <= 32)) return stream(6, 32, 2);
   auto tiles_of = [&](int bm, int bn) {
     c.bm = bm, c.tiles_m = (m + bm - 1) / bm, c.tiles_n = (d.N + bn - 1) / bn;
     c.split = 1, c.split_len = kb, c.whole = (int)c.tiles();
