@@ -128,11 +128,17 @@ def _scale_rows(scale: torch.Tensor, m: int, kb: int) -> Tuple[torch.Tensor, int
     return scale, m
 
 
+# (empty_like and empty_strided take about 1.3 us where empty takes 2.2, which a call of 6 notices)
 def _new(like: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
-    """a contiguous tensor of `like`'s shape (empty_like takes half of empty's time, but copies strides)"""
-    if like.is_contiguous():
-        return torch.empty_like(like, dtype=dtype)
-    return torch.empty(like.shape, dtype=dtype, device=like.device)
+    """a contiguous tensor of `like`'s shape"""
+    return torch.empty_like(like, dtype=dtype, memory_format=torch.contiguous_format)
+
+
+def _new_rows(lead: Sequence[int], n: int, dtype: torch.dtype, device) -> torch.Tensor:
+    """a contiguous (*lead, n) tensor"""
+    if len(lead) == 1:
+        return torch.empty_strided((lead[0], n), (n, 1), dtype=dtype, device=device)
+    return torch.empty((*lead, n), dtype=dtype, device=device)
 
 
 def _scale_strides(lead: Sequence[int], m: int) -> Tuple[int, ...]:
@@ -278,7 +284,7 @@ class BlockScaledMatmul(Operator):
         if torch.is_grad_enabled():
             _refuse_grad("BlockScaledMatmul", A, scale_a, scale_w, bias, output)
         if output is None:
-            output = torch.empty(lead + (N,), dtype=self._out, device=A.device)
+            output = _new_rows(lead, N, self._out, A.device)
         elif output.shape != lead + (N,) or output.dtype is not self._out or not output.is_contiguous() or output.get_device() != dev:
             self._refuse(A, W, scale_a, scale_w, bias, output)
         m = A.numel() // K
@@ -298,7 +304,7 @@ class BlockScaledMatmul(Operator):
         if need is None:
             need = self.workspace_bytes(m)
         if need:
-            ws = torch.empty(need, dtype=torch.uint8, device=A.device)
+            ws = torch.empty_strided((need,), (1,), dtype=torch.uint8, device=A.device)
             status = self._fn(self._ref, a_ptr, w_ptr, scale_a.data_ptr(), ld, scale_w.data_ptr(), bias_ptr, output.data_ptr(), m, ws.data_ptr(), need,
                               _raw_stream(dev))
         else:
