@@ -699,3 +699,34 @@ def test_product_last_round_in_slices(M, N, K):
     check_product(first, A, W, sa, sw, bias)
     for _ in range(3):
         assert torch.equal(op(*dev), first)
+
+
+def test_offsets_beyond_32_bits():
+    """operands, outputs and streams of more than 2^32 bytes: their last rows come out as they do alone"""
+    m, K, tail = 524288 + 300, 8208, 300
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randn(m, K, generator=g, device="cuda", dtype=torch.bfloat16)
+    last = x[-tail:].clone()
+    q, s = bitblas.quantize_blocks(x)
+    ql, sl = bitblas.quantize_blocks(last)
+    assert torch.equal(q[-tail:].view(torch.uint8), ql.view(torch.uint8)) and torch.equal(s[-tail:], sl)
+    w = torch.randn(K, generator=g, device="cuda", dtype=torch.bfloat16)
+    h, y = bitblas.residual_norm(x, x, w, 1e-5)
+    hl, yl = bitblas.residual_norm(last, last, w, 1e-5)
+    assert torch.equal(h[-tail:], hl) and torch.equal(y[-tail:], yl)
+    del h, y
+    W, sw = bitblas.quantize_blocks(x[:256], tile=True)
+    C = bitblas.BlockScaledMatmul(bitblas.BlockScaledMatmulConfig(N=256, K=K, out_dtype="bfloat16"))(q, W, s, sw)
+    check_product(C[-tail:].clone(), ql, W, sl, sw)
+    del q, s, C
+    W, sw = bitblas.quantize_blocks(x, tile=True)                         # (a tile boundary in front of the last 300 rows)
+    Wl, swl = bitblas.quantize_blocks(last, tile=True)
+    assert torch.equal(W[-tail:].view(torch.uint8), Wl.view(torch.uint8)) and torch.equal(sw[-3:], swl)
+    op = bitblas.BlockScaledMatmul(bitblas.BlockScaledMatmulConfig(N=m, K=K, out_dtype="bfloat16"))
+    for rows in (1, 40, 200):
+        A, sa = bitblas.quantize_blocks(x[:rows])
+        check_product(op(A, W, sa, sw)[:, -tail:].clone(), A, Wl, sa, swl)
+    A, sa = bitblas.quantize_blocks(x[:8200, :128].contiguous())          # an output of 8.6 GB
+    W, sw = bitblas.quantize_blocks(x[:, :128].contiguous(), tile=True)
+    C = bitblas.BlockScaledMatmul(bitblas.BlockScaledMatmulConfig(N=m, K=128, out_dtype="bfloat16"))(A, W, sa, sw)
+    check_product(C[-40:, -tail:].clone(), A[-40:], W[-tail:], sa[-40:], sw[-3:])
