@@ -35,11 +35,14 @@ Choice choose(const wqaa_block_desc& d, int m) {
   // 11.1), else two while they take a round of the chip, or up to four on short K (64 x 4096 x 4096 10.0 us against 13.7 for tiles, 64 x 6144 x 4096
   // 17.2 against 13.4; 256 x 2048 x 2048 10.0 against 12.0; 333 x 2048 x 1024, three rounds, 8.6 against 11.1;
   // 600 x 1024 x 2048 13.6 against 12.6).  Up to 32 rows there is nothing W could be shared with: 24 x 6144 x 4096 9.5 us
-  // with two, 12.0 with one; 32 x 11008 x 4096 14.6 us with four, 17.2 with two.
+  // with two, 12.0 with one; 32 x 11008 x 4096 14.6 us with four, 17.2 with two.  But where the 64-row tiles are a round of the chip or nearly,
+  // their copies through LDS ask for more of W at once: 32 x 20480 x 8192, 160 tiles, 43 us against 53 with four fragments; 24 x 28672 x 8192 50
+  // against 55; 20 x 50000 x 1024 14 against 23 (on short K two fragments stream: 24 x 22000 x 768 8.1 us, 9.7 in tiles).
   const long chunks = (m + 31) / 32, one = chunks * ((d.N + 15) / 16), two = chunks * ((d.N + 31) / 32), rounds2 = (two + 255) / 256;
   if (one <= 288 && (m <= 32 || kb <= 48)) return stream(5, 32, 1);
-  if (m <= 32 && d.N >= 10240) return stream(7, 32, 4);
-  if (m <= 32 || (rounds2 <= 4 && rounds2 * kb <= 32)) return stream(6, 32, 2);
+  const bool thin = m <= 32 && d.N < 160 * kBlock;
+  if (thin && d.N >= 10240) return stream(7, 32, 4);
+  if (thin || (rounds2 <= 4 && rounds2 * kb <= 32)) return stream(6, 32, 2);
   auto tiles_of = [&](int bm, int bn) {
     c.bm = bm, c.tiles_m = (m + bm - 1) / bm, c.tiles_n = (d.N + bn - 1) / bn;
     c.split = 1, c.split_len = kb, c.whole = (int)c.tiles();
@@ -50,31 +53,34 @@ Choice choose(const wqaa_block_desc& d, int m) {
     c.split = (kb + c.split_len - 1) / c.split_len;
     if (c.split > 1) c.whole = (int)whole;
   };
-  // many rows: the ping-pong member, a 256 x 256 tile per CU at a time.  The tiles of a last round that is not full may leave in K slices, so
-  // that it takes a half to a quarter of a round: saves 1.5 us for every k-block it is shorter, costs 0.09 us for every partial tile, to
-  // memory and back, and 6 us for the launch that adds them: 4096 x 4352 x 4096, 272 tiles, 112 us whole, 98 with the last 16 in 2
+  // many rows: the ping-pong member, a 256 x 256 tile per CU at a time.  The tiles of a last round that is not full (or of the only one) may
+  // leave in K slices, so that it takes a half to a quarter of a round: saves 1.5 us for every k-block it is shorter, costs 0.09 us for
+  // every partial tile, to memory and back, and 6 us for the launch that adds them: 4096 x 4352 x 4096, 272 tiles, 112 us whole, 98 with the last 16 in 2
   // slices, 91 in 4, 94 in 7; 4096 x 5120 x 5120, 320 tiles, 141, 136 and 126 in 4; 3000 x 8192 x 8192, 384 tiles, 236 and 223 in 2; 4096 x
-  // 9472 x 2048, 592 tiles, 115, 117 in 2, 134 in 4
+  // 9472 x 2048, 592 tiles, 115, 117 in 2, 134 in 4; 512 x 8192 x 28672, 64 tiles in 4, 123, in 128-row tiles 154
+  const long t128 = tiles_of(128, kBlock);
   const long big = tiles_of(256, 256), rounds = (big + 255) / 256, rest = big % 256;
-  if (big > 0x3fffffffl) return c;                // (block_gemm_check refuses it)
+  if (t128 > 0x3fffffffl) return c;               // (block_gemm_check refuses it)
   long split = 1, saved = 0;                      // units of 0.1 us
-  for (long z = 2; z <= 4 && rounds > 1 && rest * z <= 256; ++z) {
+  for (long z = 2; z <= 4 && rest * z <= 256; ++z) {
     const long gain = 15 * (kb - (kb + z - 1) / z) - rest * z * 9 / 10 - 60;
     if (rest > 0 && gain > saved) split = z, saved = gain;
   }
-  // taken where less than about a third of the time of its rounds is lost: 1024 x 11008 x 4096, 172 tiles, 66 us against 69 for 128-row tiles;
-  // 2048 x 10240 x 4096, 320 tiles, the last 64 in 4 slices, 110 (114 whole) against 125; 2048 x 28672 x 8192, 896 tiles, 435 against 517
-  if (m > 128 && big * 20 * 15 * kb >= 13 * 256 * (15 * kb * rounds - saved)) {
+  // taken where the tile members' rounds would take longer: a k-block of a round of 128-row tiles (two a CU) takes 1.13 us, of up to one a CU
+  // 0.62: 1100 x 8192 x 8192, 160 tiles, 105 us, 130 in 576 tiles of 128 rows; 300 x 8192 x 28672, 64 tiles in 4 slices, 116, 139 in 192;
+  // 2048 x 28672 x 8192, 896 tiles, 435, 517.  1024 x 8192 x 8192 would take 77 in 2 slices by that reckoning: 512 of 128 rows, 73
+  const long tile_time = kb * (t128 > 256 ? 113 * ((t128 + 511) / 512) : t128 >= 192 ? 62 : 62 * t128 / 192) / 10;
+  if (m > 128 && 15 * kb * rounds - saved < tile_time) {
     if (split > 1) slices(big - rest, split);
     return c;
   }
   // tiles of 128 rows where they are a tile per CU or nearly, or more than two of 64 rows per CU: 512 x 8192 x 8192, 256 of them, 43 us
   // against 50 for 512 of 64 rows; 128 x 28672 x 8192, 224 of them, 65 against 70; 700 x 8192 x 4096, 704 of 64 rows, 36 against 41
-  const long t128 = tiles_of(128, kBlock);
+  (void)tiles_of(128, kBlock);
   const bool one_each = t128 >= 192 && t128 <= 256;
   const long t64 = (long)((m + 63) / 64) * c.tiles_n;
   // 64 rows, two of them a CU, and little more than a round: that in 4 slices (333 x 11008 x 4096, 516 tiles, 35.3 us against 39.5 for 258 of 128
-  // rows; 512 x 9216 x 8192, 576 tiles, 65.3 against 67.9; 640 x 8192 x 2048, 640 tiles, 30 against 25)
+  // rows; 384 x 11264 x 4096, 528 tiles, 36.0 against 37.2; 640 x 8192 x 2048, 640 tiles, 30 against 25)
   if (m > 64 && t64 > 512 && t64 <= 512 + 64 && kb >= 32) {
     (void)tiles_of(64, kBlock);
     c.groups = 1;

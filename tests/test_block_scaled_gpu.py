@@ -730,3 +730,17 @@ def test_offsets_beyond_32_bits():
     W, sw = bitblas.quantize_blocks(x[:, :128].contiguous(), tile=True)
     C = bitblas.BlockScaledMatmul(bitblas.BlockScaledMatmulConfig(N=m, K=128, out_dtype="bfloat16"))(A, W, sa, sw)
     check_product(C[-40:, -tail:].clone(), A[-40:], W[-tail:], sa[-40:], sw[-3:])
+
+
+@pytest.mark.parametrize("M, N, K", [(300, 8190, 28688), (512, 8192, 28672), (20, 20490, 1424), (32, 28673, 2064)])
+def test_product_long_k_and_thin_batches(M, N, K):
+    """long K, where tiles of 256 rows leave in K slices; up to 32 rows against a W that fills the chip with 64-row tiles"""
+    g = torch.Generator(device="cuda").manual_seed(N)
+    A, sa = bitblas.quantize_blocks(torch.randn(M, K, generator=g, device="cuda") * torch.exp(torch.randn(K, generator=g, device="cuda")))
+    W, sw = bitblas.quantize_blocks(torch.randn(N, K, generator=g, device="cuda") * 0.05, tile=True)
+    op = bitblas.BlockScaledMatmul(bitblas.BlockScaledMatmulConfig(N=N, K=K, out_dtype="float16"))
+    plan = op.plan(M)
+    assert (plan["block_m"], plan["split_k"]) == ((256, 4) if M > 32 else (64, 1))
+    first = op(A, W, sa, sw)
+    check_product(first, A, W, sa, sw)
+    assert torch.equal(op(A, W, sa, sw), first)
