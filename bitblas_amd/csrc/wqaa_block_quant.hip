@@ -129,6 +129,7 @@ __device__ __forceinline__ float block_scale(uint32_t amax_bits, int q_dtype) {
 // x / s for 8 values of a block, rounded to 8 bits.  r = 1 / s correctly rounded once per block; x r is within an ulp of the
 // quotient, its remainder x - (x r) s is exact in one fma, and adding remainder * r gives the correctly rounded quotient
 // (P. Markstein, IBM J. Res. Dev. 34, 1990): 3 operations a value instead of a division.  s is infinite or NaN: the remainder is NaN.
+// The remainder is taken negated, n = (x r) s - x: where it vanishes n is +0, and -n r = -0 leaves x r as it is, a -0 of x's included.
 // LO: the value is v + lo, lo what v's own rounding lost; it joins the remainder.
 template <bool LO = false>
 __device__ __forceinline__ u32x2_t quantise8(const float (&v)[8], float s, int q_dtype, const float* lo = nullptr) {
@@ -137,9 +138,9 @@ __device__ __forceinline__ u32x2_t quantise8(const float (&v)[8], float s, int q
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     const float t = v[e] * r;
-    float rest = __builtin_fmaf(-t, s, v[e]);
-    if constexpr (LO) rest += lo[e];
-    q[e] = __builtin_fmaf(rest, r, t);
+    float n = __builtin_fmaf(t, s, -v[e]);
+    if constexpr (LO) n -= lo[e];
+    q[e] = __builtin_fmaf(-n, r, t);
   }
   int w[2] = {0, 0};
 #pragma unroll
