@@ -178,7 +178,8 @@ __device__ __forceinline__ float gated(float g, float u, float& lo) {
   const float e2 = __builtin_amdgcn_exp2f(t);
   const float y = 1.f + __builtin_fmaf(e2 * t_lo, 0.693147182f, e2);
   const float r0 = __builtin_amdgcn_rcpf(y);
-  const float r = t < 120.f ? __builtin_fmaf(__builtin_fmaf(-y, r0, 1.f), r0, r0) : __builtin_amdgcn_rcpf(1.f + e2);   // (2^t is or nears infinity: 0)
+  // |t| of 120 and more: 2^t is or nears infinity, r 0; or it is 0, r 1, where t_lo may have overflowed (0 t_lo a NaN)
+  const float r = __builtin_fabsf(t) < 120.f ? __builtin_fmaf(__builtin_fmaf(-y, r0, 1.f), r0, r0) : __builtin_amdgcn_rcpf(1.f + e2);
   const float c = g * r;
   const float p = c * u;
   lo = __builtin_fmaf(c, u, -p) + __builtin_fmaf(g, r, -c) * u;
