@@ -168,9 +168,10 @@ __device__ __forceinline__ void store_q(unsigned char* q, int n, u32x2_t w) {
   }
 }
 
-// silu(g) * u = u g / (1 + 2^(-g log2 e)), within about two roundings: the exponent's argument in two parts, the reciprocal with one
-// Newton step, and in `lo` what the two products round off.  (A value next to a border between two 8-bit values is decided by
-// that: with a plain exponential and reciprocal some ten times as many values fell on the other side.)
+// silu(g) * u = u g / (1 + 2^(-g log2 e)), off by 2 + 3 sigmoid(-g) roundings at most down to g = -83: the exponent's argument in two
+// parts, the reciprocal with one Newton step, and in `lo` what the two products round off.  (A value next to a border between two 8-bit
+// values is decided by that: with a plain exponential and reciprocal some ten times as many values fell on the other side.)  Below -83
+// 1 + exp(-g) is within 2^6 of leaving float32: the reciprocal is the plain one of it, and 0 from 2^126 on.
 __device__ __forceinline__ float gated(float g, float u, float& lo) {
   constexpr float kL = 1.44269502f, kLLo = 1.92596299e-8f;               // log2 e = kL + kLLo
   const float t = -g * kL;

@@ -84,3 +84,90 @@ def test_gates_where_the_exponential_leaves_float32(x):
     want = (g * torch.sigmoid(g) * 2.0 ** 94).abs()
     off = (s * 448.0 - want.clamp_min(2.0 ** -40)).abs()
     assert bool((off <= want * (8 + 2 * g.abs()) * 2.0 ** -24 + g.abs() * 2.0 ** (94 - 126) + 2.0 ** -62).all())
+
+
+U = 2.0 ** -24
+
+
+@pytest.mark.parametrize("x", list(TO))
+def test_gate_roundings(x):
+    """silu(g) u, read from the scale of blocks that hold nothing else, within 2 + 3 sigmoid(-g) roundings for the gate's sigmoid (1 + exp(-g) and its
+    reciprocal; exp(-g): one for its argument's lower part, two for a unit of the exponential) and three for the two products and the scale"""
+    n = 1 << 14
+    g = (torch.rand(n, generator=gen(21)) * 120 - 80).to(TO[x])
+    if x == "float16":
+        g = g * 0.125
+    gate, up = (torch.zeros(n, 128, dtype=TO[x]) for _ in range(2))
+    at = torch.arange(n) % 128
+    gate[torch.arange(n), at] = g
+    up[torch.arange(n), at] = (1 + torch.rand(n, generator=gen(22))).to(TO[x]) * (1.0 if x == "float16" else 2.0 ** 90)
+    s = bitblas.quantize_blocks(up.cuda(), gate=gate.cuda())[1][:, 0].cpu().double()
+    g, u = g.double(), up[torch.arange(n), at].double()
+    want = (g * torch.sigmoid(g) * u).abs()
+    keep = want > 2.0 ** -39
+    assert keep.sum() > n // 2
+    tol = want * (2 + 3 * torch.sigmoid(-g) + 3 + 0.1) * U
+    off = (s * 448.0 - want).abs()
+    assert bool((off <= tol)[keep].all()), f"worst {(off / tol)[keep].max().item():.3f} of the tolerance"
+
+
+def _near_borders(n, seed):
+    """midpoints between two neighbouring e4m3 values"""
+    g = gen(seed)
+    return (torch.randint(8, 16, (n,), generator=g) + 0.5).double() * torch.exp2(torch.randint(-8, 5, (n,), generator=g).double())
+
+
+def _steps(t, seed):
+    """float32 values moved by up to two of their own steps"""
+    move = torch.randint(-2, 3, t.shape, generator=gen(seed), dtype=torch.int32)
+    return (t.view(torch.int32) + move).view(torch.float32)
+
+
+def _check_borders(q, s, want, roundings):
+    """the bytes of `want` wherever its quotient lies further than so many roundings from a border between two 8-bit values"""
+    quotient = want / s.double()
+    step = torch.exp2(torch.floor(torch.log2(quotient.abs().clamp_min(2.0 ** -6))) - 3)
+    part = quotient.abs() / step
+    away = (part - (part.floor() + 0.5)).abs() * step / quotient.abs().clamp_min(2.0 ** -30) / U
+    value = torch.round(quotient / step) * step                             # (to even, as the 8-bit values are numbered)
+    sure = away > roundings
+    assert (sure & (away < roundings + 2)).sum() > 1000                     # (the band that a sloppier product would lose)
+    assert torch.equal(q.double()[sure], value[sure])
+
+
+def test_gated_values_next_to_borders():
+    """what the two products of silu(g) u round off counts: for g >= 32 the sigmoid is 1 and the only rounding left is the quotient's, so every value
+    further than that from a border gets the byte of the 64-bit quotient"""
+    rows = 1 << 11
+    u0 = 1 + torch.rand(rows, 1, generator=gen(31))
+    s = 32.0 * u0 / 448.0                                                   # (32 u0 is exact, and the largest of its block)
+    border = _near_borders(rows * 128, 32).view(rows, 128)
+    gate = 32 + 32 * torch.rand(rows, 128, generator=gen(33))
+    up = _steps((border * s.double() / gate.double()).float(), 34)
+    gate[:, 77], up[:, 77] = 32.0, u0[:, 0]
+    q, got = (t.cpu() for t in bitblas.quantize_blocks(up.cuda(), gate=gate.cuda()))
+    assert torch.equal(got, s)
+    _check_borders(q, s, gate.double() * up.double(), 1.1)
+
+
+def test_norm_values_next_to_borders():
+    """the same of h r w: every h is 1.5 or -1.5 and eps 0, so the mean of squares and its root are exact and r = 2 / 3 is one rounding off; the
+    quotient's is the second"""
+    D = 1 << 14
+    sign = torch.where(torch.rand(D, generator=gen(41)) < 0.5, -1.0, 1.0)
+    w0 = 1 + torch.rand(D // 128, 1, generator=gen(42))
+    s = (w0.double() / 448.0).float()
+    w = _steps((_near_borders(D, 43).view(-1, 128) * s.double()).float(), 44)
+    w[:, 5] = w0[:, 0]
+    quotients, scales, values = [], [], []
+    for i in range(16):
+        wt = torch.roll(w.view(-1), 128 * i) * 2.0 ** (i - 8)
+        y, got = bitblas.residual_norm((1.5 * sign).half().cuda()[None], None, wt.cuda(), 0.0, quantize="e4m3_float8")[1]
+        quotients.append((sign * wt).double())
+        scales.append(got.cpu().view(-1))
+        values.append(y.cpu().view(-1))
+    quotients, scales, values = torch.cat(quotients), torch.cat(scales), torch.cat(values)
+    scales = scales.repeat_interleave(128)
+    top = quotients.view(-1, 128).abs().amax(1).repeat_interleave(128)
+    assert bool(((scales.double() * 448.0 - top).abs() <= top * 4.1 * U).all())    # (r, two products, the division)
+    _check_borders(values, scales, quotients, 2.1)
