@@ -14,7 +14,7 @@ A decoder layer on this path (`BlockScaledLinear`, `BlockScaledGatedMLP`):
     out = down(act)
 
 Everything is float32 inside, with one rounding at the end, asynchronous on the current stream of the operands' device, and made for
-inference: a call that autograd would record is refused.
+inference: a call that autograd would record, backward or forward, is refused.
 """
 from __future__ import annotations
 
@@ -23,6 +23,7 @@ from dataclasses import dataclass
 from typing import Optional, Sequence, Tuple, Union
 
 import torch
+from torch.autograd import forward_ad as _forward_ad
 
 from . import lib as _lib
 from .matmul import Operator, OperatorConfig, torch_dtype
@@ -88,9 +89,17 @@ def _library():
     return _bound
 
 
+def _recorded() -> bool:
+    """whether there may be anything for `_refuse_grad` to find (forward-mode tangents do not ask for grad mode)"""
+    return torch.is_grad_enabled() or _forward_ad._current_level >= 0
+
+
 def _refuse_grad(what: str, *tensors) -> None:
-    if any(t is not None and t.requires_grad for t in tensors):
+    tensors = [t for t in tensors if t is not None]
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
         raise RuntimeError(f"{what} has no backward pass: call it under torch.no_grad(), or detach its inputs")
+    if _forward_ad._current_level >= 0 and any(_forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError(f"{what} has no forward-mode derivative: unpack its inputs")
 
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
@@ -281,8 +290,8 @@ class BlockScaledMatmul(Operator):
             if bias.dtype is not self._out or bias.shape != self._bias_shape or not bias.is_contiguous() or bias.get_device() != dev:
                 self._refuse(A, W, scale_a, scale_w, bias, output)
             bias_ptr = bias.data_ptr()
-        if torch.is_grad_enabled():
-            _refuse_grad("BlockScaledMatmul", A, scale_a, scale_w, bias, output)
+        if _recorded():
+            _refuse_grad("BlockScaledMatmul", A, W, scale_a, scale_w, bias, output)
         if output is None:
             output = _new_rows(lead, N, self._out, A.device)
         elif output.shape != lead + (N,) or output.dtype is not self._out or not output.is_contiguous() or output.get_device() != dev:
@@ -342,7 +351,7 @@ def quantize_blocks(x: torch.Tensor, dtype: str = "e4m3_float8", *, tile: bool =
         raise ValueError("tiles are taken of an (N, K) tensor, without a gate")
     if gate is not None and (gate.shape != shape or gate.dtype is not xt or gate.get_device() != dev):
         raise ValueError("gate has the shape, type and device of x")
-    if torch.is_grad_enabled():
+    if _recorded():
         _refuse_grad("quantize_blocks", x, gate, *(output or ()))
     K, lead = shape[-1], shape[:-1]
     m = x.numel() // K
@@ -461,7 +470,7 @@ def residual_norm(x: torch.Tensor, residual: Optional[torch.Tensor] = None, weig
             raise ValueError(f"quantize is one of {_FP8}, and goes with a weight")
     if not eps >= 0.0:
         raise ValueError("the norm's eps must be a non-negative number")
-    if torch.is_grad_enabled():
+    if _recorded():
         _refuse_grad("residual_norm", x, residual, weight, post_weight, gate, *(output or ()))
     passes = residual is None and gate is None and post_weight is None and scale == 1.0     # h is x
     if passes and weight is None:

@@ -209,3 +209,20 @@ def test_more_rows_than_a_launch_holds():
 def test_outputs_that_autograd_tracks_are_refused():
     with pytest.raises(RuntimeError, match="no backward"):
         bs._refuse_grad("residual_norm", torch.zeros(2), None, torch.zeros(2, requires_grad=True))
+
+
+def test_forward_mode_tangents_are_refused():
+    """also where grad mode is off, which does not switch them off; a tensor without one, and a dual tensor's primal, pass"""
+    x, v = torch.ones(2, 3), torch.ones(2, 3)
+    bs._refuse_grad("residual_norm", x, None)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(x, v)
+        for mode in (True, False):
+            with torch.set_grad_enabled(mode):
+                assert bs._recorded()
+                bs._refuse_grad("residual_norm", x, None, torch.autograd.forward_ad.unpack_dual(dual).primal, x.to(torch.float8_e4m3fn))
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    bs._refuse_grad("residual_norm", x, None, dual)
+    with torch.no_grad():
+        assert not bs._recorded()
+        bs._refuse_grad("residual_norm", torch.zeros(2, requires_grad=True))

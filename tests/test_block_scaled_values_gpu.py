@@ -171,3 +171,26 @@ def test_norm_values_next_to_borders():
     top = quotients.view(-1, 128).abs().amax(1).repeat_interleave(128)
     assert bool(((scales.double() * 448.0 - top).abs() <= top * 4.1 * U).all())    # (r, two products, the division)
     _check_borders(values, scales, quotients, 2.1)
+
+
+def test_calls_that_autograd_would_record():
+    """a weight that asks for gradients, and inputs with forward-mode tangents, are refused; without either the same call runs"""
+    x = torch.randn(4, 128, device="cuda", generator=torch.Generator("cuda").manual_seed(1)).half()
+    w = torch.ones(128, device="cuda").half()
+    q, s = bitblas.quantize_blocks(x)
+    W, sw = bitblas.quantize_blocks(x, tile=True)
+    op = bitblas.BlockScaledMatmul(bitblas.BlockScaledMatmulConfig(N=4, K=128))
+    want = op(q, W, s, sw)
+    learnt = W.clone().requires_grad_()
+    with pytest.raises(RuntimeError, match="no backward"):
+        op(q, learnt, s, sw)
+    with torch.no_grad():
+        assert torch.equal(op(q, learnt, s, sw), want)
+    ad = torch.autograd.forward_ad
+    with ad.dual_level(), torch.no_grad():
+        dual, scale, weight = ad.make_dual(x, torch.ones_like(x)), ad.make_dual(s, torch.ones_like(s)), ad.make_dual(w, w)
+        for call in (lambda: bitblas.quantize_blocks(dual), lambda: bitblas.quantize_blocks(x, gate=dual), lambda: bitblas.residual_norm(x, dual, w),
+                     lambda: bitblas.residual_norm(x, None, weight), lambda: op(q, W, scale, sw)):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+        assert torch.equal(op(q, W, s, sw), want)
