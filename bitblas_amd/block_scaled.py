@@ -558,6 +558,8 @@ class BlockScaledLinear(torch.nn.Module):
             raise ValueError(f"weight is ({self.out_features}, {self.in_features}): got {tuple(weight.shape)}")
         if (bias is not None) != (self.bias is not None):
             raise ValueError("the bias goes with a layer that has one, and only with it")
+        if bias is not None and bias.shape != (self.out_features,):
+            raise ValueError(f"bias is ({self.out_features},): got {tuple(bias.shape)}")
         w = weight.detach().to(self.weight.device)
         if w.dtype not in _FLOATS:
             w = w.float()

@@ -194,3 +194,15 @@ def test_calls_that_autograd_would_record():
             with pytest.raises(RuntimeError, match="forward-mode"):
                 call()
         assert torch.equal(op(q, W, s, sw), want)
+
+
+def test_a_bias_of_another_shape_leaves_the_layer_as_it_was():
+    """one value is no bias of 300 (a copy would spread it), and the weights of a refused call are not taken either"""
+    lin = torch.nn.Linear(128, 300, device="cuda", dtype=torch.float16)
+    layer = bitblas.BlockScaledLinear.from_linear(lin)
+    held = {k: v.clone() for k, v in layer.state_dict().items()}
+    for bias in (torch.ones(1), torch.ones(299), torch.ones(1, 300), torch.tensor(1.0)):
+        with pytest.raises(ValueError, match="bias"):
+            layer.load_float_weight(torch.zeros(300, 128), bias)
+    for name, value in layer.state_dict().items():
+        assert torch.equal(value.view(torch.uint8), held[name].view(torch.uint8))
