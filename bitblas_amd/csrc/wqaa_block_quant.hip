@@ -399,6 +399,7 @@ int block_quantize_check(const wqaa_block_quant& q) {
     set_error(WQAA_ERR_UNSUPPORTED, "block_quantize: float16 / bfloat16 / float32 to e4m3 / e5m2; a gate goes with rows only");
     return WQAA_ERR_UNSUPPORTED;
   }
+  if (q.rows > (1l << 40)) return too_many((double)q.rows, 256, "block_quantize");      // (below, rounding up leaves no 64 bits)
   const double blocks = (double)((q.K + kBlock - 1) / kBlock);
   return too_many(q.tile ? (double)((q.rows + kBlock - 1) / kBlock) * blocks : (double)((q.rows + 15) / 16) * (double)(((long)blocks + 3) / 4), 256, "block_quantize");
 }

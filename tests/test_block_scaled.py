@@ -226,3 +226,12 @@ def test_forward_mode_tangents_are_refused():
     with torch.no_grad():
         assert not bs._recorded()
         bs._refuse_grad("residual_norm", torch.zeros(2, requires_grad=True))
+
+
+@pytest.mark.parametrize("tile", [0, 1])
+@pytest.mark.parametrize("rows", [(1 << 63) - 1, (1 << 63) - 16, (1 << 41) + 1])
+def test_quantizer_row_counts_at_the_end_of_64_bits(tile, rows):
+    """a count whose rounding up to whole blocks would leave 64 bits is refused like any other that no launch holds"""
+    p = 4096
+    a = bs.BlockQuant(bs._QUANT_BYTES, wlib.BF16, wlib.E4M3, tile, rows, 128, 128, 128, rows, p, None, p, p)
+    assert bs._library().wqaa_block_quantize(ctypes.byref(a), None) == wlib.ERR_UNSUPPORTED
