@@ -235,3 +235,11 @@ def test_quantizer_row_counts_at_the_end_of_64_bits(tile, rows):
     p = 4096
     a = bs.BlockQuant(bs._QUANT_BYTES, wlib.BF16, wlib.E4M3, tile, rows, 128, 128, 128, rows, p, None, p, p)
     assert bs._library().wqaa_block_quantize(ctypes.byref(a), None) == wlib.ERR_UNSUPPORTED
+
+
+def test_member_cases_are_the_members_they_name():
+    """the device's tests of every member take what they say, whole K and cut"""
+    import test_block_scaled_members_gpu as cases
+    for name in cases.MEMBERS:
+        for cut in (False, True):
+            cases.operator(name, cut)
