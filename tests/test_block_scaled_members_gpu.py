@@ -146,3 +146,49 @@ def test_layouts(name, cut):
     out = room[13:13 + M * op.N].view(1, M, op.N)
     assert op(A[None], W, sa[None], sw, bias, out) is out
     assert torch.equal(bits(out[0]), want) and bool((room[:13] == 7).all()) and bool((room[13 + M * op.N:] == 7).all())
+
+
+@pytest.mark.parametrize("name", SLICED)
+def test_slices_on_two_streams(name):
+    """partial tiles of calls that run at once are each call's own"""
+    op, M = operator(name, out_dtype="bfloat16")
+    sets = [operands(op, M, 20 + i)[:4] for i in range(2)]
+    want = [bits(op(*s)) for s in sets]
+    assert op.workspace_bytes(M) > 0 and not torch.equal(want[0], want[1])
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(2)], [[], []]
+    for _ in range(6):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got[i].append(op(*sets[i]))
+    torch.cuda.synchronize()
+    assert all(torch.equal(bits(C), want[i]) for i in range(2) for C in got[i])
+
+
+@pytest.mark.parametrize("name", SLICED)
+def test_slices_captured(name):
+    """two graphs, each of two products that leave partial tiles, replayed on inputs that change, with the same calls made eagerly between"""
+    op, M = operator(name, out_dtype="bfloat16")
+    A, W, sa, sw, _ = operands(op, M, 30)
+    B, _, sb, _, _ = operands(op, M, 31)
+    inputs = [(A, sa), (B, sb)]
+    want = [bits(op(x, W, s, sw)) for x, s in inputs]
+    held = [[t.clone() for t in inputs[i]] for i in range(2)]
+    graphs = []
+    torch.cuda.synchronize()
+    for i in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = [op(held[i][0], W, held[i][1], sw), op(held[1 - i][0], W, held[1 - i][1], sw)]
+        graphs.append((graph, out))
+    for step in range(6):
+        swap = step // 2 % 2                                              # which input the held tensors hold
+        for i in range(2):
+            for to, now in zip(held[i], inputs[i ^ swap]):
+                to.copy_(now)
+        graph, out = graphs[step % 2]
+        graph.replay()
+        eager = bits(op(held[0][0], W, held[0][1], sw))
+        torch.cuda.synchronize()
+        i = step % 2
+        assert torch.equal(bits(out[0]), want[i ^ swap]) and torch.equal(bits(out[1]), want[1 - i ^ swap]) and torch.equal(eager, want[swap])
