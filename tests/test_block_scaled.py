@@ -243,3 +243,7 @@ def test_member_cases_are_the_members_they_name():
     for name in cases.MEMBERS:
         for cut in (False, True):
             cases.operator(name, cut)
+    for name, turns, extra in cases.TURNS:
+        M, N, member, blocks = cases.LOOPS[name]
+        plan = bitblas.BlockScaledMatmul(bitblas.BlockScaledMatmulConfig(N=N, K=turns * blocks * 128 + extra)).plan(M)
+        assert (plan["block_m"], plan["block_n"], plan["threads"]) == member, plan["name"]

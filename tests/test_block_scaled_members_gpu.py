@@ -192,3 +192,23 @@ def test_slices_captured(name):
         torch.cuda.synchronize()
         i = step % 2
         assert torch.equal(bits(out[0]), want[i ^ swap]) and torch.equal(bits(out[1]), want[1 - i ^ swap]) and torch.equal(eager, want[swap])
+
+
+# M, N, the member, and the k-blocks that its waves take in a turn of their loop
+LOOPS = {"16 x 16, 8 waves": (3, 300, (16, 16, 512), 32), "16 x 16, 16 waves": (3, 300, (16, 16, 1024), 16), "16 x 32": (9, 7300, (16, 32, 1024), 16),
+         "16 x 64": (12, 10300, (16, 64, 512), 8), "32 x 16": (30, 400, (32, 16, 512), 8), "32 x 32": (30, 7170, (32, 32, 512), 8),
+         "32 x 64": (20, 10250, (32, 64, 512), 8)}
+# the two of 16 x 16 share their calls: 16 waves from 64 blocks on
+TURNS = [(name, turns, extra) for name in LOOPS for turns in (1, 2, 3, 4, 5, 6) for extra in (-128, 0, 144)
+         if "16 x 16" not in name or (turns * LOOPS[name][3] * 128 + extra > 63 * 128) == ("16 waves" in name)]
+
+
+@pytest.mark.parametrize("name, turns, extra", TURNS)
+def test_turns_of_the_streaming_loop(name, turns, extra):
+    """K in so many turns of a wave's loop: both ways out of it, waves with a turn less, and a cut block behind"""
+    M, N, member, blocks = LOOPS[name]
+    op = bitblas.BlockScaledMatmul(bitblas.BlockScaledMatmulConfig(N=N, K=turns * blocks * 128 + extra, out_dtype="bfloat16"))
+    plan = op.plan(M)
+    assert (plan["block_m"], plan["block_n"], plan["threads"]) == member, plan["name"]
+    args = operands(op, M, turns)
+    check_product(op(*args), *args)
