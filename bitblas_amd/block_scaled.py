@@ -550,6 +550,16 @@ class BlockScaledLinear(torch.nn.Module):
         else:
             self.bias = None
 
+    def _apply(self, fn, *args, **kw):
+        """`.to()`, `.half()`, `.cuda()` and the like move the buffers and leave their types alone: those are the operator's, and a 16-bit scale or
+        weight could not be turned back"""
+        held = {name: t for name, t in self._buffers.items() if t is not None}
+        super()._apply(fn, *args, **kw)
+        for name, t in held.items():
+            if self._buffers[name].dtype is not t.dtype:
+                self._buffers[name] = t.to(self._buffers[name].device)
+        return self
+
     def load_float_weight(self, weight: torch.Tensor, bias: Optional[torch.Tensor] = None) -> None:
         """Quantise a float weight into this layer's buffers, on the GPU the layer lives on."""
         if self.weight.device.type != "cuda":

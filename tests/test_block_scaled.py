@@ -247,3 +247,20 @@ def test_member_cases_are_the_members_they_name():
         M, N, member, blocks = cases.LOOPS[name]
         plan = bitblas.BlockScaledMatmul(bitblas.BlockScaledMatmulConfig(N=N, K=turns * blocks * 128 + extra)).plan(M)
         assert (plan["block_m"], plan["block_n"], plan["threads"]) == member, plan["name"]
+
+
+@pytest.mark.parametrize("change", [lambda m: m.half(), lambda m: m.bfloat16(), lambda m: m.double(), lambda m: m.to(torch.float32), lambda m: m.to("meta", torch.bfloat16),
+                                    lambda m: m.to(torch.zeros(1, dtype=torch.float16))], ids=["half", "bfloat16", "double", "float", "meta", "like"])
+def test_a_model_cast_leaves_the_layer_its_types(change):
+    """a cast of the model around it: the operator still takes the layer's buffers, and their values are whole"""
+    lin = bitblas.BlockScaledLinear(256, 128, bias=True, W_dtype="e5m2_float8", out_dtype="bfloat16")
+    lin.weight.view(torch.uint8).copy_(torch.arange(256, dtype=torch.uint8).expand(128, 256) & 0x3F)
+    lin.weight_scale.fill_(2.0 ** -40 / 448)
+    lin.bias.fill_(3.0)
+    held = {k: v.clone() for k, v in lin.state_dict().items()}
+    model = torch.nn.Sequential(lin, torch.nn.Linear(4, 4))
+    assert change(model) is model
+    for name, was in held.items():
+        now = getattr(lin, name)
+        assert now.dtype == was.dtype and now.shape == was.shape and now is lin.state_dict(keep_vars=True)[name]
+        assert now.device.type == "meta" or torch.equal(now.view(torch.uint8), was.view(torch.uint8))
