@@ -114,14 +114,18 @@ def _rows(t: torch.Tensor) -> Tuple[torch.Tensor, int]:
     if t.dim() == 2 and t.stride(1) == 1 and t.stride(0) >= k:
         return t, t.stride(0)
     if t.dim() >= 2 and t.stride(-1) == 1:
-        ld = t.stride(-2)
-        step = ld
+        ld = step = None
         for size, stride in zip(t.shape[-2::-1], t.stride()[-2::-1]):
-            if size != 1 and stride != step:
+            if size == 1:
+                continue
+            if step is None:
+                ld, step = stride, stride * size
+            elif stride == step:
+                step *= size
+            else:
                 break
-            step *= size
         else:
-            if ld >= k:
+            if ld is not None and ld >= k:
                 return t, ld
     t = t.contiguous()
     return t, k

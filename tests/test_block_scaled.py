@@ -264,3 +264,18 @@ def test_a_model_cast_leaves_the_layer_its_types(change):
         now = getattr(lin, name)
         assert now.dtype == was.dtype and now.shape == was.shape and now is lin.state_dict(keep_vars=True)[name]
         assert now.device.type == "meta" or torch.equal(now.view(torch.uint8), was.view(torch.uint8))
+
+
+def test_rows_with_axes_of_one_between():
+    """the last token of each sequence, (B, 1, K): rows as even as without the axis of one, and read where they are"""
+    t = torch.arange(4 * 6 * 10).view(4, 6, 10)
+    for view, ld in ((t[:, -1:], 60), (t[:, 2:3, 1:8], 60), (t[:, None, 3, :5], 60), (t.view(4, 6, 1, 10)[::2, :, :, :4][:1], 10), (t[1:3, :, None, 2:], 10)):
+        assert not view.is_contiguous()
+        got, d = bs._rows(view)
+        k = view.shape[-1]
+        assert d == ld and got.data_ptr() == view.data_ptr()
+        assert torch.equal(torch.as_strided(got, (view.numel() // k, k), (d, 1), got.storage_offset()), view.reshape(-1, k))
+    for view in (t[:, 1:2, ::2], t[:, :2].transpose(0, 1)[:, None], t[:1, None].expand(4, 1, 6, 10)):
+        got, d = bs._rows(view)
+        k = view.shape[-1]
+        assert torch.equal(torch.as_strided(got, (view.numel() // k, k), (d, 1), got.storage_offset()), view.reshape(-1, k))
