@@ -95,11 +95,13 @@ def _recorded() -> bool:
 
 
 def _refuse_grad(what: str, *tensors) -> None:
-    tensors = [t for t in tensors if t is not None]
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
-        raise RuntimeError(f"{what} has no backward pass: call it under torch.no_grad(), or detach its inputs")
-    if _forward_ad._current_level >= 0 and any(_forward_ad.unpack_dual(t).tangent is not None for t in tensors):
-        raise RuntimeError(f"{what} has no forward-mode derivative: unpack its inputs")
+    for t in tensors:
+        if t is not None and t.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError(f"{what} has no backward pass: call it under torch.no_grad(), or detach its inputs")
+    if _forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and _forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError(f"{what} has no forward-mode derivative: unpack its inputs")
 
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
