@@ -79,8 +79,10 @@ Choice choose(const wqaa_block_desc& d, int m) {
   (void)tiles_of(128, kBlock);
   const bool one_each = t128 >= 192 && t128 <= 256;
   const long t64 = (long)((m + 63) / 64) * c.tiles_n;
-  // 64 rows, two of them a CU, and little more than a round: that in 4 slices (333 x 11008 x 4096, 516 tiles, 35.3 us against 39.5 for 258 of 128
-  // rows; 384 x 11264 x 4096, 528 tiles, 36.0 against 37.2; 640 x 8192 x 2048, 640 tiles, 30 against 25)
+  // 64 rows, two of them a CU, and little more than a round: that in 4 slices, which fill the chip once up to 64 tiles (of K = 4096, in slices against
+  // tiles of 128 rows: 384 x 11008, 516 tiles, 33.4 us against 37.6; 384 x 11520, 540, 33.7 and 38.0; 1000 x 4480, 560, 33.6 and 35.3; 384 x 12032,
+  // 564, 34.1 and 38.2; 640 x 7296, 570, 35.2 and 38.5; 384 x 12288, 576, 34.3 and 34.7; beyond: 384 x 12800, 600, 38.7 and 38.4; 640 x 7680, 600, 39.4
+  // and 38.6; 384 x 13568, 636, 40.0 and 38.7; 640 x 8192, 640, 39.7 and 34.2.  From about K = 8192 on the 256-row tiles above take these)
   if (m > 64 && t64 > 512 && t64 <= 512 + 64 && kb >= 32) {
     (void)tiles_of(64, kBlock);
     c.groups = 1;

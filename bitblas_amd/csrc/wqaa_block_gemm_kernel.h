@@ -63,7 +63,9 @@ __device__ __forceinline__ void block_store4(void* C, int dt, long i, int n, con
 // from L2 - the same way; the waves' partial tiles meet in LDS in a fixed order.  Rows beyond m and n repeat the last one and are
 // not stored.  Workgroups along y take 16 MF rows each.  U blocks are asked for at once; PF: the next U before the matrix
 // instructions of these.  NF > 1 divides the reads of the activations, which at 16 rows are as many as those of the weights (choose() in
-// wqaa_block_gemm.hip has the measured rule).  One row, 28672 x 8192: 38.6 us, 6.1 TB/s; 16 rows, 8192 x 28672: 46 us, 5.1 TB/s.
+// wqaa_block_gemm.hip has the measured rule).  With more weights in turn than
+// the last-level cache holds, 2 GB of them: one row, 28672 x 8192, 38.5 us, 6.1 TB/s; 16 rows, 8192 x 28672, 46 us, 5.1 TB/s (one and the same operands
+// again and again: 37.3 and 39.6).
 template <int WF, int AF, int WAVES, int U, int NF, int MF, bool PF>
 __global__ void __launch_bounds__(WAVES * 64) wq_block_stream_kernel(const BlockGemmArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
