@@ -186,7 +186,7 @@ def _scale_ld(scale: torch.Tensor, lead: Sequence[int], m: int, kb: int) -> int:
 
 @dataclass(frozen=True)
 class BlockScaledMatmulConfig(OperatorConfig):
-    """One block-scaled product: A (M, K) x W (N, K)^T, any row count."""
+    """One block-scaled product: A (M, K) x W (N, K)^T, any row count; K a multiple of 16 up to 2^22."""
     N: int = None
     K: int = None
     A_dtype: str = "e4m3_float8"
@@ -335,8 +335,8 @@ def quantize_blocks(x: torch.Tensor, dtype: str = "e4m3_float8", *, tile: bool =
                     output: Optional[Tuple[torch.Tensor, torch.Tensor]] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """(values, scales) of x in blocks of 128 along its last axis.
 
-    x       (..., K) in float16, bfloat16 or float32; rows may lie apart (a slice of a wider tensor).  K is any number here; a product
-            wants a multiple of 16
+    x       (..., K) in float16, bfloat16 or float32; rows may lie apart (a slice of a wider tensor).  K is any number up to 2^30 here; a
+            product wants a multiple of 16
     tile    False: a scale per row and block, (..., ceil(K / 128)) - activations.  True: x is (N, K) and a scale stands for 128 rows
             too, (ceil(N / 128), ceil(K / 128)) - weights
     gate    as x: silu(gate) * x is quantised, computed in float32 and not rounded in between (rows only)

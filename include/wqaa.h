@@ -417,7 +417,7 @@ int wqaa_peer_exchange(const wqaa_peer_exchange_desc* desc, void* stream);
 
 /* ---- block-scaled 8-bit floating point: both operands in e4m3 / e5m2, one float32 scale per block of 128 consecutive k ----------
  * C[m, n] = sum_b scale_a(m, b) scale_w(n / 128, b) sum_{k in block b} A[m, k] W[n, k]  (+ bias[n]), one rounding to out_dtype.
- * A: (m, K) bytes, W: (N, K) bytes, both row-major; K a multiple of 16, the last block may hold fewer than 128 k; any N >= 1.
+ * A: (m, K) bytes, W: (N, K) bytes, both row-major; K a multiple of 16 up to 2^22, the last block may hold fewer than 128 k; any N >= 1.
  * scale_a: the scale of (row m, block b) at scale_a[b * scale_a_ld + m], scale_a_ld >= m (the rows of one block side by side: what
  * wqaa_block_quantize writes); scale_w: (ceil(N / 128), ceil(K / 128)) row-major; bias: (N,) of out_dtype when with_bias.
  * Sums are float32, but for the matrix unit's own: of 8 consecutive k it adds the products with what each has below 2^-13 of the largest
@@ -443,7 +443,7 @@ int wqaa_block_select(const wqaa_block_desc* desc, int m, wqaa_plan* plan);
  * largest value of q_dtype (448, 57344); q = x / s, the float32 quotient, rounded to nearest even.  A block that holds an infinity or
  * a NaN gets a scale that is not finite, and NaN in all its values.  gate != NULL: x = silu(gate) * X, in float32.
  * X, gate: (rows, K) with rows x_ld / gate_ld elements apart; Q: (rows, K) bytes, contiguous; S: (row, block) at S[block * s_ld + row], s_ld >= rows,
- * or, for tiles, (ceil(rows / 128), ceil(K / 128)) row-major (s_ld is not read).  Any K >= 1. */
+ * or, for tiles, (ceil(rows / 128), ceil(K / 128)) row-major (s_ld is not read).  1 <= K <= 2^30.  Zeros keep their sign. */
 typedef struct wqaa_block_quant {
   int32_t struct_size;   /* = sizeof(wqaa_block_quant) */
   int32_t x_dtype;       /* WQAA_F16 / WQAA_BF16 / WQAA_F32, of X and gate */
